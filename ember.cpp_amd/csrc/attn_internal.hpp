@@ -1,0 +1,81 @@
+// Internal declarations shared by the cache and attention translation units (not part of the C ABI).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ember_attn.h"
+
+namespace ember_attn_impl {
+
+// n / d for 0 <= n < 2^31 by a multiplication and a shift (Granlund and Montgomery, 1994): a page may hold any
+// number of tokens, and every lane divides.
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+__device__ inline uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return (__umulhi(n, f.mul) + n) >> f.shift;
+}
+
+// A call's cache and batch as the kernels take them.
+struct CacheArgs {
+  void *k, *v;
+  _Float16 *ks, *vs;       // Q8_0 scales
+  int type, n_kv, D, n_pages;
+  FastDiv page;            // tokens per page
+  // the batch
+  int n_seqs, n_tokens, max_q;
+  int cap;                 // tokens that a sequence can have: max_kv, and what its pages hold
+  int max_pages;           // row width of `pages`
+  const int32_t* q_start;  // or null
+  const int32_t* kv_len;
+  const int32_t* pages;    // or null
+};
+
+// Index of the cache row (page, KV head 0, row in the page) in units of [page] rows of one head: the page's first row
+// is pid * n_kv * page. -1: no such page.
+__device__ inline int64_t cache_row(const CacheArgs& c, int b, int pos) {
+  const uint32_t pg = div_by((uint32_t)pos, c.page);
+  const int pid = c.pages ? c.pages[(int64_t)b * c.max_pages + pg] : b;
+  if ((uint32_t)pid >= (uint32_t)c.n_pages) return -1;
+  return (int64_t)pid * c.n_kv * c.page.d + (pos - (int)(pg * c.page.d));
+}
+__device__ inline int seq_len(const CacheArgs& c, int b) { return max(0, min(c.kv_len[b], c.cap)); }
+
+// Rows of sequence b: first row and count, kept inside [0, n_tokens).
+__device__ inline void seq_rows(const CacheArgs& c, int b, int& first, int& count) {
+  if (!c.q_start) {
+    first = b;
+    count = 1;
+    return;
+  }
+  first = c.q_start[b];
+  const int end = min(c.q_start[b + 1], c.n_tokens);
+  count = first < 0 ? 0 : max(0, end - first);
+}
+
+int make_cache_args(const ember_kv_cache* c, const ember_kv_batch* b, CacheArgs* out);
+
+int launch_kv_store(const CacheArgs& c, const void* k, int64_t ks, const void* v, int64_t vs, int type, hipStream_t st);
+int launch_kv_load(const CacheArgs& c, void* k, int64_t ks, void* v, int64_t vs, int type, hipStream_t st);
+
+struct AttnArgs {
+  CacheArgs c;
+  int H, G;                // heads, heads per KV head
+  float scale, softcap;
+  int window;              // 0: none
+  const float* slopes;     // or null
+  const int32_t* prefix;   // or null
+  int shared;
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;
+  int type;                // of q and out
+};
+int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st);
+
+}  // namespace ember_attn_impl

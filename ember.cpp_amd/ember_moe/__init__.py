@@ -136,6 +136,8 @@ def lib() -> ctypes.CDLL:
         L.ember_gguf_layer_bytes.restype = sz
         L.ember_gguf_upload_layer.argtypes = [ctypes.POINTER(GgufMoe), vp, sz, ctypes.POINTER(Layer), vp]
         L.ember_gguf_upload_layer.restype = i
+        attention.declare(L)
+        sampling.declare(L)
         _lib = L
     return _lib
 
@@ -602,3 +604,11 @@ def gguf_upload_layer(m: GgufMoe, dev, stream=None) -> Layer:
         raise EmberError(st, "ember_gguf_upload_layer")
     L._owner = dev
     return L
+
+
+# ----------------------------------------------------------------------------------------------
+# The cache, the attention over it and the pick of the next token (include/ember_attn.h, ember_sample.h)
+
+from . import attention, sampling  # noqa: E402
+from .attention import AttnOpts, DeviceKvCache, KvBatch, KvCache, attn_options, kv_batch  # noqa: E402,F401
+from .sampling import Sampler, sample  # noqa: E402,F401

@@ -1,0 +1,218 @@
+"""Python binding of the paged cache and the attention over it (include/ember_attn.h), on torch tensors.
+
+A decoder layer keeps its keys and values in a `DeviceKvCache`; `kv_batch` says which sequences a step works on and where
+their tokens lie; `store` puts the step's new rows into the cache, `attend` computes the attention of the new tokens over
+all of it, `load` reads rows back. Errors raise EmberError with the status that the C entry gives (or would give, for what
+only the binding can see: tensor types, shapes and devices).
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+from typing import Optional
+
+import ember_moe as em
+
+
+class KvCache(ctypes.Structure):
+    """ember_kv_cache (include/ember_attn.h)."""
+
+    _fields_ = [("type", ctypes.c_int), ("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int), ("page", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+
+
+class KvBatch(ctypes.Structure):
+    """ember_kv_batch (include/ember_attn.h)."""
+
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_q", ctypes.c_int), ("max_kv", ctypes.c_int),
+                ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("max_pages", ctypes.c_int), ("shared", ctypes.c_int)]
+
+
+class AttnOpts(ctypes.Structure):
+    """ember_attn_opts (include/ember_attn.h)."""
+
+    _fields_ = [("n_heads", ctypes.c_int), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("window", ctypes.c_int), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
+
+
+def declare(L: ctypes.CDLL) -> None:
+    vp, i, i64, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+    cp, bp, ap = ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), ctypes.POINTER(AttnOpts)
+    for f in (L.ember_kv_store, L.ember_kv_load):
+        f.argtypes, f.restype = [cp, bp, vp, i64, vp, i64, i, vp], i
+    L.ember_attn_scratch_bytes.argtypes, L.ember_attn_scratch_bytes.restype = [ap, cp, bp], sz
+    L.ember_attn.argtypes, L.ember_attn.restype = [ap, cp, bp, vp, i64, vp, i64, i, vp, sz, vp], i
+
+
+_IDS: dict = {}
+
+
+def type_id(t) -> int:
+    """The ggml type id of a tensor's dtype (F32, F16, BF16)."""
+    if not _IDS:
+        import torch
+
+        _IDS.update({torch.float32: em.F32, torch.float16: em.F16, torch.bfloat16: em.BF16})
+    ty = _IDS.get(t.dtype)
+    if ty is None:
+        raise em.EmberError(em.ERR_TYPE, f"dtype {t.dtype}")
+    return ty
+
+
+def on_current_device(t) -> None:
+    """Refuses tensors that are not on the current device: the library launches there."""
+    import torch
+
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise em.EmberError(em.ERR_LAUNCH, f"tensor on {t.device}, the current device is another")
+
+
+def _array(t, n: int, dtype, what: str) -> int:
+    """The address of a caller's device array of n values, or 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.numel() < n or not t.is_contiguous():
+        raise em.EmberError(em.ERR_SHAPE, f"{what}: a contiguous {dtype} tensor of {n} values is needed")
+    return t.data_ptr()
+
+
+def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: int = 1, max_kv: int = 0, pages=None,
+             shared: int = 0) -> KvBatch:
+    """A batch's descriptor from int32 device tensors: kv_len [n_seqs], q_start [n_seqs + 1] (None: one new token
+    each), pages [n_seqs, max_pages] (None: sequence b lies in page b). Keeps the tensors."""
+    import torch
+
+    n = kv_len.numel()
+    b = KvBatch(n_seqs=n, n_tokens=n if n_tokens is None else n_tokens, max_q=max_q, max_kv=max_kv, shared=shared)
+    b.kv_len = _array(kv_len, n, torch.int32, "kv_len")
+    b.q_start = _array(q_start, n + 1, torch.int32, "q_start")
+    if pages is not None:
+        if pages.dim() != 2 or pages.shape[0] < n:
+            raise em.EmberError(em.ERR_SHAPE, "pages: [n_seqs, max_pages] is needed")
+        b.pages, b.max_pages = _array(pages, pages.numel(), torch.int32, "pages"), pages.shape[1]
+    for t in (kv_len, q_start, pages):
+        if t is not None:
+            on_current_device(t)
+    b._owner = (kv_len, q_start, pages)
+    return b
+
+
+def attn_options(n_heads: int, head_dim: int, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                 slopes=None, prefix=None) -> AttnOpts:
+    """Attention options; scale None: 1 / sqrt(head_dim). slopes f32 [n_heads], prefix int32 [n_seqs]. Keeps the tensors."""
+    import torch
+
+    a = AttnOpts(n_heads=n_heads, scale=head_dim ** -0.5 if scale is None else scale, softcap=softcap, window=window)
+    a.slopes = _array(slopes, n_heads, torch.float32, "slopes")
+    a.prefix = _array(prefix, 0, torch.int32, "prefix")
+    for t in (slopes, prefix):
+        if t is not None:
+            on_current_device(t)
+    a._owner = (slopes, prefix)
+    return a
+
+
+def _rows(t, n: int, heads: int, dim: int, what: str) -> int:
+    """Checks a [n, heads, dim] tensor whose rows may be apart (a slice of a joint projection); its row stride."""
+    if t.dim() != 3 or t.shape[0] < n or t.shape[1] != heads or t.shape[2] != dim or (heads > 1 and t.stride(1) != dim) or t.stride(2) != 1:
+        raise em.EmberError(em.ERR_SHAPE, f"{what}: [{n}, {heads}, {dim}] with whole rows is needed, got {tuple(t.shape)}")
+    # (a single row's stride is anyone's: torch may give 1)
+    return max(t.stride(0), heads * dim) if n <= 1 else t.stride(0)
+
+
+@dataclass
+class DeviceKvCache:
+    """One layer's cache on the device: k, v [n_pages, n_kv, page, head_dim] (int8 with fp16 k_scale, v_scale [n_pages,
+    n_kv, page, head_dim / 32] for Q8_0) and the C descriptor pointing at them."""
+
+    type: int
+    k: object
+    v: object
+    k_scale: object = None
+    v_scale: object = None
+    desc: KvCache = field(default_factory=KvCache)
+
+    def __post_init__(self):
+        import torch
+
+        want = {em.F16: torch.float16, em.BF16: torch.bfloat16, em.Q8_0: torch.int8}.get(self.type)
+        if want is None:
+            raise em.EmberError(em.ERR_TYPE, "a cache is F16, BF16 or Q8_0")
+        shape = tuple(self.k.shape)
+        if len(shape) != 4 or tuple(self.v.shape) != shape or not self.k.is_contiguous() or not self.v.is_contiguous():
+            raise em.EmberError(em.ERR_SHAPE, "k, v: contiguous [n_pages, n_kv, page, head_dim] are needed")
+        if self.k.dtype != want or self.v.dtype != want:
+            raise em.EmberError(em.ERR_TYPE, f"k, v of a {em.TYPE_NAMES[self.type]} cache are {want}")
+        d = self.desc
+        d.type, (d.n_pages, d.n_kv, d.page, d.head_dim) = self.type, shape
+        d.k, d.v = self.k.data_ptr(), self.v.data_ptr()
+        for t in (self.k, self.v):
+            on_current_device(t)
+        if self.type == em.Q8_0:
+            for t in (self.k_scale, self.v_scale):
+                if t is None or tuple(t.shape) != shape[:3] + (shape[3] // 32,) or t.dtype != torch.float16 or not t.is_contiguous():
+                    raise em.EmberError(em.ERR_SHAPE, "k_scale, v_scale: contiguous fp16 [n_pages, n_kv, page, head_dim / 32] are needed")
+                on_current_device(t)
+            d.k_scale, d.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
+
+    @staticmethod
+    def create(type_: int, n_pages: int, n_kv: int, page: int, head_dim: int, device="cuda") -> "DeviceKvCache":
+        import torch
+
+        dt = {em.F16: torch.float16, em.BF16: torch.bfloat16, em.Q8_0: torch.int8}.get(type_)
+        if dt is None:
+            raise em.EmberError(em.ERR_TYPE, "a cache is F16, BF16 or Q8_0")
+        shape = (n_pages, n_kv, page, head_dim)
+        k, v = (torch.zeros(shape, dtype=dt, device=device) for _ in range(2))
+        if type_ != em.Q8_0:
+            return DeviceKvCache(type_, k, v)
+        return DeviceKvCache(type_, k, v, *(torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.float16, device=device) for _ in range(2)))
+
+    def _kv(self, fn: str, batch: KvBatch, k, v, stream):
+        d = self.desc
+        ks, vs = (_rows(t, batch.n_tokens, d.n_kv, d.head_dim, n) for t, n in ((k, "k"), (v, "v")))
+        if k.dtype != v.dtype:
+            raise em.EmberError(em.ERR_TYPE, "k and v of one type are needed")
+        for t in (k, v):
+            on_current_device(t)
+        st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, type_id(k), em._stream(stream))
+        if st:
+            raise em.EmberError(st, fn)
+        return k, v
+
+    def store(self, batch: KvBatch, k, v, stream=None) -> None:
+        """Stores rows k, v [n_tokens, n_kv, head_dim] (f32, f16 or bf16) at the batch's places (ember_kv_store)."""
+        self._kv("ember_kv_store", batch, k, v, stream)
+
+    def load(self, batch: KvBatch, k, v, stream=None):
+        """Reads the rows at the batch's places into k, v (ember_kv_load); returns them."""
+        return self._kv("ember_kv_load", batch, k, v, stream)
+
+    def attn_scratch_bytes(self, opts: AttnOpts, batch: KvBatch) -> int:
+        return int(em.lib().ember_attn_scratch_bytes(ctypes.byref(opts), ctypes.byref(self.desc), ctypes.byref(batch)))
+
+    def attend(self, opts: AttnOpts, batch: KvBatch, q, out=None, scratch=None, stream=None):
+        """Attention of the rows q [n_tokens, n_heads, head_dim] over the cache (ember_attn); returns out."""
+        import torch
+
+        d = self.desc
+        qs = _rows(q, batch.n_tokens, opts.n_heads, d.head_dim, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        os_ = _rows(out, batch.n_tokens, opts.n_heads, d.head_dim, "out")
+        if out.dtype != q.dtype:
+            raise em.EmberError(em.ERR_TYPE, "q and out of one type are needed")
+        prefix = getattr(opts, "_owner", (None, None))[1]
+        if prefix is not None and prefix.numel() < batch.n_seqs:
+            raise em.EmberError(em.ERR_SHAPE, "prefix: one length per sequence is needed")
+        for t in (q, out) if scratch is None else (q, out, scratch):
+            on_current_device(t)
+        if scratch is None:
+            scratch = torch.empty(max(1, self.attn_scratch_bytes(opts, batch)), dtype=torch.uint8, device=q.device)
+        st = em.lib().ember_attn(ctypes.byref(opts), ctypes.byref(d), ctypes.byref(batch), q.data_ptr(), qs, out.data_ptr(), os_,
+                                 type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream))
+        if st:
+            raise em.EmberError(st, "ember_attn")
+        return out
