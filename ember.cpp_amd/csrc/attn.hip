@@ -1,6 +1,7 @@
-// Attention over the paged cache (ember_attn).
-#include "attn_internal.hpp"
-#include "moe_conv.hpp"
+// Attention over the paged cache (ember_attn): which kernels a call takes, and the join of its parts.
+#include <algorithm>
+
+#include "attn_dev.hpp"
 
 namespace ember_attn_impl {
 namespace {
@@ -76,10 +77,90 @@ __global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
   }
 }
 
+// Rows of parts (Parts) as output rows: a wave per row. Its lanes first hold one part's maximum and sum each, then the row's columns.
+template <int IO>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts) {
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int tok = at / a.H, h = at - tok * a.H;
+  int first, count;
+  seq_rows(c, blockIdx.y, first, count);
+  if (tok >= min(count, c.max_q)) return;
+  const int64_t row = (int64_t)(first + tok) * a.H + h;
+  float M = kNoScore;
+  for (int p = lane; p < parts.n; p += 64) M = fmaxf(M, parts.ml[(p * parts.rows + row) * 2]);
+  for (int k = 32; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+  float sum = 0.0f;
+  f4 x = {0, 0, 0, 0};
+  const int d = lane * 4;
+  for (int p0 = 0; p0 < parts.n; p0 += 64) {
+    float w = 0.0f, l = 0.0f;
+    if (p0 + lane < parts.n) {
+      const float* ml = parts.ml + ((p0 + lane) * parts.rows + row) * 2;
+      l = ml[1];
+      w = exp2_fast(ml[0] - M);
+    }
+    sum += l * w;
+    for (uint64_t todo = __ballot(l != 0.0f); todo; todo &= todo - 1) {  // (parts without a visible key hold nothing)
+      const int p = __ffsll((unsigned long long)todo) - 1;
+      const float wp = __shfl(w, p);
+      if (d < c.D) {
+        f4 y = *reinterpret_cast<const f4*>(parts.o + ((p0 + p) * parts.rows + row) * c.D + d);
+        y *= wp;
+        x += y;
+      }
+    }
+  }
+  for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  x *= inv;
+  const u2 y = {pack2<IO == EMBER_TYPE_BF16>(x[0], x[1]), pack2<IO == EMBER_TYPE_BF16>(x[2], x[3])};
+  if (d < c.D) *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
+}
+
 }  // namespace
 
-int launch_attn(const AttnArgs& a, void*, hipStream_t st) {
-  attn_row_kernel<<<dim3(a.c.max_q, a.H, a.c.n_seqs), 64, 0, st>>>(a);
+AttnPlan attn_plan(const AttnArgs& a) {
+  AttnPlan p{};
+  const CacheArgs& c = a.c;
+  p.step = (int64_t)c.max_q * a.G <= 64;
+  if (!p.step) return p;
+  // keys that the rows of a sequence can see at most, and one tile for where they begin within one
+  int64_t range = c.cap;
+  if (a.window > 0 && !a.prefix) range = std::min<int64_t>(range, (int64_t)a.window + c.max_q - 1);
+  range = std::max<int64_t>(range, 1) + 31;
+  const int64_t blocks = (int64_t)c.n_seqs * c.n_kv * ((c.max_q * a.G + 15) / 16);
+  const int64_t most = (range + 127) / 128;
+  int64_t splits = std::min<int64_t>({most, 256, (2048 + blocks - 1) / blocks});
+  p.chunk = (int)((range + splits - 1) / splits + 127) / 128 * 128;
+  p.splits = (int)((range + p.chunk - 1) / p.chunk);
+  p.parts = p.splits > 1 ? p.splits : 0;
+  return p;
+}
+
+size_t attn_scratch(const AttnArgs& a) {
+  const AttnPlan p = attn_plan(a);
+  return (size_t)p.parts * a.c.n_tokens * a.H * (a.c.D + 2) * 4;
+}
+
+int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st) {
+  const AttnPlan p = attn_plan(a);
+  if (!p.step) {
+    attn_row_kernel<<<dim3(a.c.max_q, a.H, a.c.n_seqs), 64, 0, st>>>(a);
+    return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
+  }
+  Parts parts{nullptr, nullptr, (int64_t)a.c.n_tokens * a.H, std::max(p.parts, 1)};
+  if (p.parts) {
+    parts.o = static_cast<float*>(scratch);
+    parts.ml = parts.o + p.parts * parts.rows * a.c.D;
+  }
+  auto* step = a.c.type == EMBER_TYPE_BF16 ? launch_step_bf16 : a.c.type == EMBER_TYPE_F16 ? launch_step_f16
+               : a.type == EMBER_TYPE_BF16 ? launch_step_q8_bf16 : launch_step_q8_f16;
+  if (int s = step(a, parts, p.splits, p.chunk, 0, st)) return s;
+  if (!p.parts) return EMBER_OK;
+  const dim3 grid(((unsigned)a.c.max_q * a.H + 3) / 4, a.c.n_seqs);
+  if (a.type == EMBER_TYPE_BF16) attn_join_kernel<EMBER_TYPE_BF16><<<grid, 256, 0, st>>>(a, parts);
+  else attn_join_kernel<EMBER_TYPE_F16><<<grid, 256, 0, st>>>(a, parts);
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }
 

@@ -14,8 +14,8 @@ int check_cache(const ember_kv_cache* c) {
   if (c->type != EMBER_TYPE_F16 && c->type != EMBER_TYPE_BF16 && c->type != EMBER_TYPE_Q8_0) return EMBER_ERR_TYPE;
   if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32 || c->n_kv < 1 || c->n_kv > 256 || c->page < 1 || c->n_pages < 1)
     return EMBER_ERR_SHAPE;
-  // (every index of a value fits 48 bits: more memory than there is)
-  if ((double)c->n_pages * c->page * c->n_kv * c->head_dim > 2.8e14) return EMBER_ERR_SHAPE;
+  // rows of one head are numbered by 32 bits
+  if ((double)c->n_pages * c->page * c->n_kv >= 4294967295.0) return EMBER_ERR_SHAPE;
   const bool q8 = c->type == EMBER_TYPE_Q8_0;
   if (!c->k || !c->v || (q8 && (!c->k_scale || !c->v_scale))) return EMBER_ERR_NULL;
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || (q8 && (!aligned(c->k_scale, 16) || !aligned(c->v_scale, 16)))) return EMBER_ERR_ALIGN;
@@ -24,7 +24,7 @@ int check_cache(const ember_kv_cache* c) {
 
 int check_batch(const ember_kv_cache* c, const ember_kv_batch* b) {
   if (!b) return EMBER_ERR_NULL;
-  if (b->n_seqs < 0 || b->n_seqs > 65535 || b->n_tokens < 0 || b->max_q < 1 || b->max_kv < 0 || b->max_kv > (1 << 30) || b->shared < 0)
+  if (b->n_seqs < 0 || b->n_seqs > 65535 || b->n_tokens < 0 || b->max_q < 1 || b->max_kv < 0 || b->max_kv > (1 << 29) || b->shared < 0)
     return EMBER_ERR_SHAPE;
   if (!b->q_start && b->n_tokens < b->n_seqs) return EMBER_ERR_SHAPE;
   if (b->pages ? b->max_pages < 1 : (b->n_seqs > c->n_pages || b->shared)) return EMBER_ERR_SHAPE;
@@ -123,8 +123,8 @@ int ember_kv_load(const ember_kv_cache* c, const ember_kv_batch* b, void* k, int
 }
 
 size_t ember_attn_scratch_bytes(const ember_attn_opts* a, const ember_kv_cache* c, const ember_kv_batch* b) {
-  if (check_attn(a, c, b)) return 0;
-  return 0;
+  if (check_attn(a, c, b) || b->n_seqs == 0 || b->n_tokens == 0) return 0;
+  return attn_scratch(attn_args(a, c, b));
 }
 
 int ember_attn(const ember_attn_opts* a, const ember_kv_cache* c, const ember_kv_batch* b, const void* q, int64_t q_stride,

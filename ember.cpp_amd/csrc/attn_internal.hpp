@@ -76,6 +76,21 @@ struct AttnArgs {
   int64_t q_stride, out_stride;
   int type;                // of q and out
 };
+// How a call runs, by its sizes alone: attn_step_kernel for up to 64 rows per KV head and sequence; the keys of a sequence in
+// `splits` parts of `chunk`.
+struct AttnPlan {
+  bool step;
+  int splits, chunk;
+  int parts;  // parts in the scratch, 0 where the kernel writes the output itself
+};
+AttnPlan attn_plan(const AttnArgs& a);
+size_t attn_scratch(const AttnArgs& a);
 int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st);
+
+struct Parts;
+int launch_step_bf16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_f16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_q8_bf16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_q8_f16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
 
 }  // namespace ember_attn_impl

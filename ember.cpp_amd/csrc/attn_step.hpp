@@ -1,0 +1,365 @@
+// Attention of a few new tokens per sequence (tiles of 16 query rows per KV head) over the cache; instantiated per cache type by
+// attn_step_*.hip.
+//
+// Bound by the cache's bytes: every key and value is read once, for all heads that share it. A block takes one KV head of one
+// sequence (and one part of its keys, where sequences are few or long: the parts are joined by attn_join_kernel), its four
+// waves take tiles of 32 keys in turn, each on its own: no barrier until the waves' results are joined at the end. A tile's
+// rows are loaded in whole rows into registers while the tile before it is computed, and pass through LDS, which K leaves as
+// the matrix cores' A operand and V transposed. 16 query rows fill an operand's columns; with 4 heads per KV head three quarters
+// of it are idle, which costs nothing while the loads take longer. More rows than 16 are tiles of their own, which read the cache again.
+#pragma once
+#include "attn_dev.hpp"
+
+namespace ember_attn_impl {
+
+constexpr int kStepThreads = 256, kStepWaves = 4, kTile = 32;
+
+template <int T, int DP>
+struct StepLds {
+  static constexpr int kCH = DP * Op<T>::kBytes / 16;
+  static constexpr int kTileBytes = kTile * kCH * 16;
+  static constexpr int kScaleBytes = Op<T>::kQ8 ? (DP / 32) * kTile * 2 : 0;
+  static constexpr int kWave = 2 * kTileBytes + kScaleBytes;
+  static constexpr int kJoin = 16 * DP * 4;  // a wave's result
+  static constexpr int kPerWave = kWave > kJoin ? kWave : kJoin;
+  static constexpr int kBytes = kStepWaves * kPerWave;
+};
+
+// A wave's loads of one tile: rows of K and V, in order, 16 bytes a lane.
+template <int T, int DP>
+struct TileRegs {
+  static constexpr int kCH = DP * Op<T>::kBytes / 16, kN = kCH / 2;
+  u4 k[kN], v[kN];
+  u4 ks[2];        // Q8_0: the scales of this lane's two keys (l % 16, 16 + l % 16), for K
+  u4 vs;           // and of key l % 32, for V
+};
+
+template <int T, int IO, int DP, bool GEN>
+__global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_kernel(AttnArgs a, Parts parts, int tiles, int chunk, int begin) {
+  using O = Op<T>;
+  using L = StepLds<T, DP>;
+  constexpr int CH = L::kCH, NL = CH / 2, KS = DP / 32, DT = DP / 16;
+  extern __shared__ __attribute__((aligned(256))) char lds[];
+  const CacheArgs& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n16 = lane & 15;
+  const int split = blockIdx.x / tiles, r0 = (blockIdx.x - split * tiles) * 16, kvh = blockIdx.y, b = blockIdx.z;
+  int first, count;
+  seq_rows(c, b, first, count);
+  const int nrows = min(16, min(count, c.max_q) * a.G - r0);  // rows of this tile: r0 + n is head n % G of token n / G
+  if (nrows <= 0) return;
+  const int len = seq_len(c, b), total = c.q_start ? c.q_start[b + 1] - first : 1;
+  const int64_t p0 = (int64_t)len - total;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  // positions of the tile's first and last row, keys that any of its rows sees, and keys that all see
+  const int64_t pa = p0 + r0 / a.G, pz = p0 + (r0 + nrows - 1) / a.G;
+  const Span sa = visible(a, pa, len, prefix), sz = visible(a, pz, len, prefix);
+  const int lo = max(visible(a, max(pa, (int64_t)0), len, prefix).lo, begin), hi = sz.hi;
+  const int all_lo = sz.lo, all_hi = sa.hi;  // (none where the first row is before the first position)
+  const int k0 = (lo & ~(kTile - 1)) + split * chunk, k1 = min(hi, k0 + chunk);
+
+  // the query rows as B operands: column n16, and for step s the columns of d that K's operand holds in this lane
+  s8 qf[KS];
+  float c_row, slope;
+  Span see;
+  int pos;
+  {
+    const int r = r0 + n16, tok = r / a.G, h = kvh * a.G + (r - tok * a.G);
+    const bool ok = n16 < nrows;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (ok ? (int64_t)(first + tok) * a.q_stride + (int64_t)h * c.D : 0);
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = O::kQ8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 32 * s + 8 * g;
+      qf[s] = s8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (ok && d < c.D) qf[s] = *reinterpret_cast<const s8*>(q + d);
+      if constexpr (IO == EMBER_TYPE_BF16 && !O::kBf16)
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(ember_moe::bf16_f32((uint16_t)qf[s][i])));
+    }
+    float mul = a.scale * (GEN && a.softcap > 0.0f ? 2.0f / a.softcap : 1.0f) * kLog2e;
+    if constexpr (IO == EMBER_TYPE_BF16 && !O::kBf16) {
+      // bf16 queries as fp16: each row by a power of two that puts its largest value into [0.5, 1), undone in the scores; exact but
+      // for values under 2^-14 of the largest, whose last bits go
+      top = max_lanes32(max_lanes16(top));
+      int e = 0;
+      if (top > 0.0f && top <= 3.4028235e38f) (void)__builtin_frexpf(top, &e);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        h8 x;
+        for (int i = 0; i < 8; ++i) x[i] = (_Float16)__builtin_ldexpf(ember_moe::bf16_f32((uint16_t)qf[s][i]), -e);
+        qf[s] = __builtin_bit_cast(s8, x);
+      }
+      mul = fminf(__builtin_ldexpf(mul, e), 3e38f);
+    }
+    c_row = mul;
+    see = ok ? visible(a, p0 + tok, len, prefix) : Span{0, INT32_MAX};
+    pos = (int)(p0 + tok);
+    slope = GEN && a.slopes && ok ? a.slopes[h] * kLog2e : 0.0f;
+  }
+  const float cap = GEN && a.softcap > 0.0f ? a.softcap * kLog2e : 0.0f;
+
+  f4 o[DT];
+  float m = kNoScore, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = f4{0, 0, 0, 0};
+
+  char* const kt_ = lds + wave * L::kPerWave;
+  char* const vt_ = kt_ + L::kTileBytes;
+  _Float16* const vs_ = reinterpret_cast<_Float16*>(vt_ + L::kTileBytes);
+  const int ch = c.D * O::kBytes / 16;  // chunks of a row (CH with columns past D, which are zero)
+
+  // cache row (kvh's) of key kt + lane % 32, clamped into the sequence; ~0: in no page
+  auto look_up = [&](int kt) -> uint32_t {
+    const int j = min(kt + (lane & 31), hi - 1);
+    const int64_t r = cache_row(c, b, j);
+    return r < 0 ? ~0u : (uint32_t)(r + (int64_t)kvh * c.page.d);
+  };
+  TileRegs<T, DP> reg;
+  auto load = [&](uint32_t rows) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
+      uint32_t row = __shfl(rows, key);
+      row = row == ~0u ? 0 : row;
+      const int64_t at = (int64_t)row * c.D * O::kBytes + cc * 16;
+      reg.k[i] = reg.v[i] = u4{0, 0, 0, 0};
+      if (cc < ch) {
+        reg.k[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.k) + at);
+        reg.v[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.v) + at);
+      }
+    }
+    if constexpr (O::kQ8) {
+      const int nb = c.D / 32;
+      auto scales = [&](const _Float16* p, uint32_t row) {
+        row = row == ~0u ? 0 : row;
+        union { u4 w; _Float16 h[8]; } x;
+        x.w = u4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          if (i < nb) x.h[i] = p[(int64_t)row * nb + i];
+        return x.w;
+      };
+      reg.ks[0] = scales(c.ks, __shfl(rows, n16));
+      reg.ks[1] = scales(c.ks, __shfl(rows, 16 + n16));
+      reg.vs = scales(c.vs, rows);
+    }
+  };
+
+  int kt = k0 + wave * kTile;
+  uint32_t rows = 0, rows_next = 0;
+  if (kt < k1) {
+    rows = look_up(kt);
+    load(rows);
+    rows_next = look_up(kt + kStepWaves * kTile);
+  }
+  for (; kt < k1; kt += kStepWaves * kTile) {
+    // values of keys outside the rows' span count for none of them, whatever they hold
+    const bool inside = kt >= lo && kt + kTile <= hi;
+    bool odd = false;  // a value in this lane that is not finite
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
+      *reinterpret_cast<u4*>(kt_ + k_at<CH>(key, cc)) = reg.k[i];
+      u4 v = reg.v[i];
+      if (!inside && (kt + key < lo || kt + key >= hi)) v = u4{0, 0, 0, 0};
+      *reinterpret_cast<u4*>(vt_ + v_at<CH, O::kQ8>(key, cc)) = v;
+      if constexpr (!O::kQ8) {
+        constexpr uint32_t e = O::kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd |= (v[w] & e) == e || (v[w] & (e << 16)) == (e << 16);
+      }
+    }
+    h8 k_scale[2];
+    if constexpr (O::kQ8) {
+      union { u4 w; _Float16 h[8]; } x;
+      x.w = reg.vs;
+      if (lane < 32) {
+        const bool out = kt + lane < lo || kt + lane >= hi;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          const _Float16 sc = out ? (_Float16)0.0f : x.h[i];
+          vs_[i * kTile + lane] = sc;
+          odd |= (__builtin_bit_cast(uint16_t, sc) & 0x7c00u) == 0x7c00u;
+        }
+      }
+      k_scale[0] = __builtin_bit_cast(h8, reg.ks[0]);
+      k_scale[1] = __builtin_bit_cast(h8, reg.ks[1]);
+    }
+    const uint32_t here = rows;
+    // the next tile's loads, over this tile's registers
+    if (kt + kStepWaves * kTile < k1) {
+      rows = rows_next;
+      load(rows);
+      rows_next = look_up(kt + 2 * kStepWaves * kTile);
+    }
+
+    f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = half * 16 + n16;
+      if constexpr (O::kQ8) {
+#pragma unroll
+        for (int u = 0; u < KS / 2; ++u) {
+          const u4 w = *reinterpret_cast<const u4*>(kt_ + k_at<CH>(key, g + 4 * u));
+          const _Float16 sc = g < 2 ? k_scale[half][2 * u] : k_scale[half][2 * u + 1];
+          const h8 s8_ = {sc, sc, sc, sc, sc, sc, sc, sc};
+          const s8 x = codes_times(u2{w[0], w[1]}, s8_), y = codes_times(u2{w[2], w[3]}, s8_);
+          s[half] = mma16<false>(x, qf[2 * u], s[half]);
+          s[half] = mma16<false>(y, qf[2 * u + 1], s[half]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < KS; ++u) {
+          const s8 x = *reinterpret_cast<const s8*>(kt_ + k_at<CH>(key, 4 * u + g));
+          s[half] = mma16<O::kBf16>(x, qf[u], s[half]);
+        }
+      }
+    }
+
+    const bool masked = kt < all_lo || kt + kTile > all_hi || kt < lo || kt + kTile > hi;
+    const bool torn = __ballot(here == ~0u) != 0;  // keys in no page: their scores are NaN
+    uint32_t bad = 0;
+    if (torn) bad = (uint32_t)__ballot(here == ~0u);
+    const Scores sc{c_row, cap, slope};
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = (i >> 2) * 16 + g * 4 + (i & 3);
+      x[i] = GEN ? sc(s[i >> 2][i & 3], kt + key - pos) : s[i >> 2][i & 3] * c_row;
+      if (torn && (bad >> key & 1)) x[i] = __builtin_nanf("");
+      if (masked && (kt + key < max(see.lo, lo) || kt + key >= min(see.hi, hi))) x[i] = -INFINITY;
+    }
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    top = max_lanes32(max_lanes16(top));
+    // the maximum moves only when it is left behind by more than 2^8: weights then stay below 2^8, well inside fp16, and the
+    // sums are seldom rescaled
+    if (__ballot(top > m + 8.0f)) {
+      const float m2 = fmaxf(m, top), al = exp2_fast(m - m2);
+      m = m2;
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= al;
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = exp2_fast(x[i] - m);
+    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    const s8 pf = __builtin_bit_cast(s8, u4{pack2<O::kBf16>(w[0], w[1]), pack2<O::kBf16>(w[2], w[3]), pack2<O::kBf16>(w[4], w[5]),
+                                            pack2<O::kBf16>(w[6], w[7])});
+
+    auto v_frag = [&](int d) -> s8 {
+      if constexpr (O::kQ8) {
+        const int j = n16 >> 1, key = (j & 3) + (j >> 2) * 16 + g * 4;
+        const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((EMBER_LDS(i2)*)(vt_ + v_at<CH, true>(key, d) + (n16 & 1) * 8));
+        const u2 a0 = *reinterpret_cast<const u2*>(vs_ + (d >> 1) * kTile + g * 4);
+        const u2 a1 = *reinterpret_cast<const u2*>(vs_ + (d >> 1) * kTile + 16 + g * 4);
+        return codes_times(u2{(uint32_t)w[0], (uint32_t)w[1]}, __builtin_bit_cast(h8, u4{a0[0], a0[1], a1[0], a1[1]}));
+      } else {
+        const int key = g * 4 + (n16 >> 2), cc = 2 * d + ((n16 >> 1) & 1);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key, cc) + (n16 & 1) * 8));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key + 16, cc) + (n16 & 1) * 8));
+        return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      }
+    };
+    if (masked && pa != pz && __ballot(odd)) {
+      // a value that is not finite among keys that some rows see and others do not (their weight 0 times it were NaN): it
+      // counts as 0 in the sum, and the rows that see it get NaN in its column
+      const short one = O::kBf16 ? (short)0x3f80 : (short)0x3c00, ex = O::kBf16 ? (short)0x7f80 : (short)0x7c00;
+      s8 vis;
+      for (int i = 0; i < 8; ++i) {
+        const int key = kt + (i >> 2) * 16 + g * 4 + (i & 3);
+        vis[i] = key >= max(see.lo, lo) && key < min(see.hi, hi) ? one : (short)0;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const s8 v = v_frag(d);
+        s8 flag, fine;
+        for (int i = 0; i < 8; ++i) {
+          const bool f = (v[i] & ex) == ex;
+          flag[i] = f ? one : (short)0;
+          fine[i] = f ? (short)0 : v[i];
+        }
+        const f4 hit = mma16<O::kBf16>(flag, vis, f4{0, 0, 0, 0});
+        o[d] = mma16<O::kBf16>(fine, pf, o[d]);
+        for (int i = 0; i < 4; ++i)
+          if (hit[i] > 0.0f) o[d][i] = __builtin_nanf("");
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] = mma16<O::kBf16>(v_frag(d), pf, o[d]);
+    }
+  }
+
+  // the four waves' results as one
+  __shared__ float wm[kStepWaves][16], wl[kStepWaves][16];
+  __syncthreads();
+  l = sum_lanes32(sum_lanes16(l));
+  if (g == 0) {
+    wm[wave][n16] = m;
+    wl[wave][n16] = l;
+  }
+  __syncthreads();
+  float* const join = reinterpret_cast<float*>(lds + wave * L::kPerWave);
+  {
+    float M = wm[0][n16];
+    for (int w = 1; w < kStepWaves; ++w) M = fmaxf(M, wm[w][n16]);
+    const float al = exp2_fast(m - M);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      f4 x = o[d];
+      x *= al;
+      *reinterpret_cast<f4*>(join + n16 * DP + d * 16 + g * 4) = x;
+    }
+  }
+  __syncthreads();
+  // 4 columns of a row per thread
+  for (int at = threadIdx.x; at < nrows * (DP / 4); at += kStepThreads) {
+    const int r = at / (DP / 4), d = (at % (DP / 4)) * 4;
+    if (d >= c.D) continue;
+    float M = wm[0][r], sum = 0.0f;
+    for (int w = 1; w < kStepWaves; ++w) M = fmaxf(M, wm[w][r]);
+    f4 x = {0, 0, 0, 0};
+    for (int w = 0; w < kStepWaves; ++w) {
+      sum += wl[w][r] * exp2_fast(wm[w][r] - M);
+      x += *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(lds + w * L::kPerWave) + r * DP + d);
+    }
+    const int tok = (r0 + r) / a.G, h = kvh * a.G + (r0 + r - tok * a.G);
+    if (parts.o) {
+      const int64_t row = (int64_t)split * parts.rows + (int64_t)(first + tok) * a.H + h;
+      *reinterpret_cast<f4*>(parts.o + row * c.D + d) = x;
+      if (d == 0) {
+        parts.ml[row * 2] = M;
+        parts.ml[row * 2 + 1] = sum;
+      }
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      x *= inv;
+      const u2 y = {pack2<IO == EMBER_TYPE_BF16>(x[0], x[1]), pack2<IO == EMBER_TYPE_BF16>(x[2], x[3])};
+      *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
+    }
+  }
+}
+
+template <int T, int IO, int DP>
+int launch_step(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st) {
+  const int tiles = (a.c.max_q * a.G + 15) / 16;
+  const dim3 grid(splits * tiles, a.c.n_kv, a.c.n_seqs);
+  const size_t lds = StepLds<T, DP>::kBytes;
+  auto go = [&](auto* kernel) {
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
+      return (int)EMBER_ERR_LAUNCH;
+    kernel<<<grid, kStepThreads, lds, st>>>(a, p, tiles, chunk, begin);
+    return hipGetLastError() == hipSuccess ? (int)EMBER_OK : (int)EMBER_ERR_LAUNCH;
+  };
+  return a.softcap > 0.0f || a.slopes ? go(attn_step_kernel<T, IO, DP, true>) : go(attn_step_kernel<T, IO, DP, false>);
+}
+
+template <int T, int IO>
+int launch_step_type(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st) {
+  if (a.c.D <= 64) return launch_step<T, IO, 64>(a, p, splits, chunk, begin, st);
+  if (a.c.D <= 128) return launch_step<T, IO, 128>(a, p, splits, chunk, begin, st);
+  return launch_step<T, IO, 256>(a, p, splits, chunk, begin, st);
+}
+
+}  // namespace ember_attn_impl

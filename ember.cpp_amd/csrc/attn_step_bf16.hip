@@ -1,0 +1,8 @@
+// attn_step.hpp for BF16 caches and BF16 rows.
+#include "attn_step.hpp"
+
+namespace ember_attn_impl {
+int launch_step_bf16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st) {
+  return launch_step_type<EMBER_TYPE_BF16, EMBER_TYPE_BF16>(a, p, splits, chunk, begin, st);
+}
+}  // namespace ember_attn_impl

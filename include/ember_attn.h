@@ -31,7 +31,7 @@ extern "C" {
  *   Q8_0       k, v [n_pages][n_kv][page][head_dim] int8 codes, and per 32 of them one fp16 scale in k_scale, v_scale
  *              [n_pages][n_kv][page][head_dim / 32]: the numbers of ggml's Q8_0 blocks in two planes, so that rows
  *              stay 16-byte aligned
- * head_dim: a multiple of 32 from 32 to 256. n_kv <= 256. All pointers 16-byte aligned. */
+ * head_dim: a multiple of 32 from 32 to 256. n_kv <= 256, n_pages * n_kv * page < 2^32 - 1. All pointers 16-byte aligned. */
 typedef struct ember_kv_cache {
   int type;
   int n_kv, head_dim, page, n_pages;
@@ -51,7 +51,7 @@ typedef struct ember_kv_batch {
   int n_seqs;               /* up to 65535 */
   int n_tokens;             /* rows of q, k, v and out */
   int max_q;                /* no sequence has more new tokens (those past max_q get no attention output) */
-  int max_kv;               /* no sequence has more tokens in the cache */
+  int max_kv;               /* no sequence has more tokens in the cache; up to 1 << 29 */
   const int32_t* q_start;   /* [n_seqs + 1] device, ascending, or NULL: one token each, n_tokens >= n_seqs */
   const int32_t* kv_len;    /* [n_seqs] device */
   const int32_t* pages;     /* [n_seqs][max_pages] device, or NULL */
