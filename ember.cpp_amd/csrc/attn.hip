@@ -6,77 +6,6 @@
 namespace ember_attn_impl {
 namespace {
 
-__device__ inline float load_half(const void* p, int64_t at, int type) {
-  return type == EMBER_TYPE_F16 ? (float)static_cast<const _Float16*>(p)[at] : ember_moe::bf16_f32(static_cast<const uint16_t*>(p)[at]);
-}
-__device__ inline float cached(const CacheArgs& c, const void* p, const _Float16* scales, int64_t row, int d) {
-  if (c.type == EMBER_TYPE_Q8_0) return (float)static_cast<const int8_t*>(p)[row * c.D + d] * (float)scales[row * (c.D / 32) + d / 32];
-  return load_half(p, row * c.D + d, c.type);
-}
-
-// One wave per (new token, head): lanes over the keys of a 64-key tile for the scores, over the head's columns for the
-// weighted sum; the running maximum and sum of the softmax in f32.
-__global__ __launch_bounds__(64) void attn_row_kernel(AttnArgs a) {
-  const CacheArgs& c = a.c;
-  const int b = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x, D = c.D;
-  __shared__ float qs[256], ps[64];
-  __shared__ int64_t rows[64];
-  int first, count;
-  seq_rows(c, b, first, count);
-  if (i >= count) return;
-  const int len = seq_len(c, b), total = c.q_start ? c.q_start[b + 1] - first : 1;
-  const int64_t p = (int64_t)len - total + i;
-  const int kvh = h / a.G;
-  const int64_t q_at = (int64_t)(first + i) * a.q_stride + (int64_t)h * D;
-  for (int d = lane; d < D; d += 64) qs[d] = load_half(a.q, q_at + d, a.type);
-  const int prefix = a.prefix ? a.prefix[b] : 0;
-  const float slope = a.slopes ? a.slopes[h] : 0.0f;
-  const int64_t lo = a.window > 0 ? max((int64_t)0, p - a.window + 1) : 0;
-  const int64_t hi = p < 0 ? 0 : min((int64_t)len, max(p + 1, (int64_t)prefix));
-  float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
-  __syncthreads();
-  for (int64_t j0 = lo; j0 < hi; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const bool seen = j < hi;
-    const int64_t row = seen ? cache_row(c, b, (int)j) : -1;
-    float s = -INFINITY;
-    if (seen) {
-      s = __builtin_nanf("");
-      if (row >= 0) {
-        s = 0.0f;
-        for (int d = 0; d < D; ++d) s += qs[d] * cached(c, c.k, c.ks, row + (int64_t)kvh * c.page.d, d);
-        s *= a.scale;
-        if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-        if (a.slopes) s -= slope * fabsf((float)(p - j));
-      }
-    }
-    float t = s;
-    for (int k = 32; k; k >>= 1) t = fmaxf(t, __shfl_xor(t, k));
-    const float m2 = fmaxf(m, t), base = m2 == -INFINITY ? 0.0f : m2;
-    const float w = expf(s - base), alpha = expf(m - base);
-    float sum = w;
-    for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-    l = l * alpha + sum;
-    m = m2;
-    ps[lane] = w;
-    rows[lane] = row;
-    __syncthreads();
-    const int n = (int)min((int64_t)64, hi - j0);
-    for (int u = 0; u * 64 + lane < D; ++u) {
-      o[u] *= alpha;
-      for (int k = 0; k < n; ++k)
-        if (rows[k] >= 0) o[u] += ps[k] * cached(c, c.v, c.vs, rows[k] + (int64_t)kvh * c.page.d, u * 64 + lane);
-    }
-    __syncthreads();
-  }
-  const int64_t out_at = (int64_t)(first + i) * a.out_stride + (int64_t)h * D;
-  for (int u = 0; u * 64 + lane < D; ++u) {
-    const float r = l == 0.0f ? 0.0f : o[u] / l;
-    if (a.type == EMBER_TYPE_F16) static_cast<_Float16*>(a.out)[out_at + u * 64 + lane] = (_Float16)r;
-    else static_cast<uint16_t*>(a.out)[out_at + u * 64 + lane] = ember_moe::bf16_rne(r);
-  }
-}
-
 // Rows of parts (Parts) as output rows: a wave per row. Its lanes first hold one part's maximum and sum each, then the row's columns.
 template <int IO>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts) {
@@ -123,18 +52,23 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts)
 AttnPlan attn_plan(const AttnArgs& a) {
   AttnPlan p{};
   const CacheArgs& c = a.c;
-  p.step = (int64_t)c.max_q * a.G <= 64;
-  if (!p.step) return p;
+  const int64_t rows = (int64_t)c.max_q * a.G;
+  p.step = rows <= 64;
+  p.begin = std::min(a.shared, c.cap);
+  auto split = [](int64_t keys, int64_t blocks, int64_t want, int unit, int& splits, int& chunk) {
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({keys / unit, 256, (want + blocks - 1) / blocks}));
+    chunk = (int)((keys + n * unit - 1) / (n * unit)) * unit;
+    splits = (int)((keys + chunk - 1) / chunk);
+  };
   // keys that the rows of a sequence can see at most, and one tile for where they begin within one
-  int64_t range = c.cap;
+  int64_t range = c.cap - p.begin;
   if (a.window > 0 && !a.prefix) range = std::min<int64_t>(range, (int64_t)a.window + c.max_q - 1);
-  range = std::max<int64_t>(range, 1) + 31;
-  const int64_t blocks = (int64_t)c.n_seqs * c.n_kv * ((c.max_q * a.G + 15) / 16);
-  const int64_t most = (range + 127) / 128;
-  int64_t splits = std::min<int64_t>({most, 256, (2048 + blocks - 1) / blocks});
-  p.chunk = (int)((range + splits - 1) / splits + 127) / 128 * 128;
-  p.splits = (int)((range + p.chunk - 1) / p.chunk);
-  p.parts = p.splits > 1 ? p.splits : 0;
+  range = std::max<int64_t>(range, 1) + 63;
+  const int64_t groups = (int64_t)c.n_seqs * c.n_kv;
+  if (p.step) split(range, groups * ((rows + 15) / 16), 2048, 128, p.splits, p.chunk);
+  else split(range, groups * ((rows + 127) / 128), 512, 256, p.splits, p.chunk);
+  if (p.begin) split(p.begin, c.n_kv * (((int64_t)c.n_tokens * a.G + 127) / 128), 512, 256, p.shared_splits, p.shared_chunk);
+  p.parts = p.splits + p.shared_splits > 1 ? p.splits + p.shared_splits : 0;
   return p;
 }
 
@@ -145,20 +79,21 @@ size_t attn_scratch(const AttnArgs& a) {
 
 int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st) {
   const AttnPlan p = attn_plan(a);
-  if (!p.step) {
-    attn_row_kernel<<<dim3(a.c.max_q, a.H, a.c.n_seqs), 64, 0, st>>>(a);
-    return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
-  }
   Parts parts{nullptr, nullptr, (int64_t)a.c.n_tokens * a.H, std::max(p.parts, 1)};
   if (p.parts) {
     parts.o = static_cast<float*>(scratch);
     parts.ml = parts.o + p.parts * parts.rows * a.c.D;
   }
-  auto* step = a.c.type == EMBER_TYPE_BF16 ? launch_step_bf16 : a.c.type == EMBER_TYPE_F16 ? launch_step_f16
-               : a.type == EMBER_TYPE_BF16 ? launch_step_q8_bf16 : launch_step_q8_f16;
-  if (int s = step(a, parts, p.splits, p.chunk, 0, st)) return s;
-  if (!p.parts) return EMBER_OK;
-  const dim3 grid(((unsigned)a.c.max_q * a.H + 3) / 4, a.c.n_seqs);
+  const int kind = a.c.type == EMBER_TYPE_BF16 ? 0 : a.c.type == EMBER_TYPE_F16 ? 1 : a.type == EMBER_TYPE_BF16 ? 2 : 3;
+  decltype(&launch_step_bf16) const steps[4] = {launch_step_bf16, launch_step_f16, launch_step_q8_bf16, launch_step_q8_f16};
+  decltype(&launch_wide_bf16) const wides[4] = {launch_wide_bf16, launch_wide_f16, launch_wide_q8_bf16, launch_wide_q8_f16};
+  int s = EMBER_OK;
+  if (p.begin) s = wides[kind](a, parts, WideCall{0, p.shared_splits, p.shared_chunk, 0, p.begin}, st);
+  if (s) return s;
+  if (p.step) s = steps[kind](a, parts, p.shared_splits, p.splits, p.chunk, p.begin, st);
+  else s = wides[kind](a, parts, WideCall{p.shared_splits, p.splits, p.chunk, p.begin, 0}, st);
+  if (s || !p.parts) return s;
+  const dim3 grid((unsigned)(((int64_t)a.c.max_q * a.H + 3) / 4), a.c.n_seqs);
   if (a.type == EMBER_TYPE_BF16) attn_join_kernel<EMBER_TYPE_BF16><<<grid, 256, 0, st>>>(a, parts);
   else attn_join_kernel<EMBER_TYPE_F16><<<grid, 256, 0, st>>>(a, parts);
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;

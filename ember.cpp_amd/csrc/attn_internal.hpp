@@ -76,11 +76,13 @@ struct AttnArgs {
   int64_t q_stride, out_stride;
   int type;                // of q and out
 };
-// How a call runs, by its sizes alone: attn_step_kernel for up to 64 rows per KV head and sequence; the keys of a sequence in
-// `splits` parts of `chunk`.
+// How a call runs, by its sizes alone. Every sequence's keys from `begin` on: attn_step_kernel for up to 64 rows per KV head and
+// sequence, attn_wide_kernel for more, in `splits` parts of `chunk` keys; before that the shared pages (begin > 0), the batch's
+// rows together, in shared_splits of shared_chunk.
 struct AttnPlan {
   bool step;
   int splits, chunk;
+  int begin, shared_splits, shared_chunk;
   int parts;  // parts in the scratch, 0 where the kernel writes the output itself
 };
 AttnPlan attn_plan(const AttnArgs& a);
@@ -88,9 +90,18 @@ size_t attn_scratch(const AttnArgs& a);
 int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st);
 
 struct Parts;
-int launch_step_bf16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
-int launch_step_f16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
-int launch_step_q8_bf16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
-int launch_step_q8_f16(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st);
+// `part0`: the first of the parts that a launch writes
+int launch_step_bf16(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_f16(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_q8_bf16(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st);
+int launch_step_q8_f16(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st);
+// A launch of attn_wide_kernel: its parts begin with part0; end > 0: the shared pages, up to there.
+struct WideCall {
+  int part0, splits, chunk, begin, end;
+};
+int launch_wide_bf16(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st);
+int launch_wide_f16(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st);
+int launch_wide_q8_bf16(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st);
+int launch_wide_q8_f16(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st);
 
 }  // namespace ember_attn_impl

@@ -35,7 +35,7 @@ struct TileRegs {
 };
 
 template <int T, int IO, int DP, bool GEN>
-__global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_kernel(AttnArgs a, Parts parts, int tiles, int chunk, int begin) {
+__global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_kernel(AttnArgs a, Parts parts, int part0, int tiles, int chunk, int begin) {
   using O = Op<T>;
   using L = StepLds<T, DP>;
   constexpr int CH = L::kCH, NL = CH / 2, KS = DP / 32, DT = DP / 16;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
     }
     const int tok = (r0 + r) / a.G, h = kvh * a.G + (r0 + r - tok * a.G);
     if (parts.o) {
-      const int64_t row = (int64_t)split * parts.rows + (int64_t)(first + tok) * a.H + h;
+      const int64_t row = (int64_t)(part0 + split) * parts.rows + (int64_t)(first + tok) * a.H + h;
       *reinterpret_cast<f4*>(parts.o + row * c.D + d) = x;
       if (d == 0) {
         parts.ml[row * 2] = M;
@@ -342,24 +342,24 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
 }
 
 template <int T, int IO, int DP>
-int launch_step(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st) {
+int launch_step(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st) {
   const int tiles = (a.c.max_q * a.G + 15) / 16;
   const dim3 grid(splits * tiles, a.c.n_kv, a.c.n_seqs);
   const size_t lds = StepLds<T, DP>::kBytes;
   auto go = [&](auto* kernel) {
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
       return (int)EMBER_ERR_LAUNCH;
-    kernel<<<grid, kStepThreads, lds, st>>>(a, p, tiles, chunk, begin);
+    kernel<<<grid, kStepThreads, lds, st>>>(a, p, part0, tiles, chunk, begin);
     return hipGetLastError() == hipSuccess ? (int)EMBER_OK : (int)EMBER_ERR_LAUNCH;
   };
   return a.softcap > 0.0f || a.slopes ? go(attn_step_kernel<T, IO, DP, true>) : go(attn_step_kernel<T, IO, DP, false>);
 }
 
 template <int T, int IO>
-int launch_step_type(const AttnArgs& a, const Parts& p, int splits, int chunk, int begin, hipStream_t st) {
-  if (a.c.D <= 64) return launch_step<T, IO, 64>(a, p, splits, chunk, begin, st);
-  if (a.c.D <= 128) return launch_step<T, IO, 128>(a, p, splits, chunk, begin, st);
-  return launch_step<T, IO, 256>(a, p, splits, chunk, begin, st);
+int launch_step_type(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st) {
+  if (a.c.D <= 64) return launch_step<T, IO, 64>(a, p, part0, splits, chunk, begin, st);
+  if (a.c.D <= 128) return launch_step<T, IO, 128>(a, p, part0, splits, chunk, begin, st);
+  return launch_step<T, IO, 256>(a, p, part0, splits, chunk, begin, st);
 }
 
 }  // namespace ember_attn_impl

@@ -1,0 +1,403 @@
+// Attention of many query rows over the cache: prompts, and the pages that a whole batch shares; instantiated per cache type by
+// attn_wide_*.hip.
+//
+// Bound by the matrix cores. A block takes 128 query rows of one KV head (the heads that share it are rows too, so their keys
+// are loaded once), 32 for each of its four waves, and goes through the keys in tiles that all waves read from LDS. The next tile's
+// rows are loaded into registers while this one is computed, and stored to the other half of the LDS (quantised rows as fp16:
+// converted once for all four waves); one barrier per tile. 32 x 32 x 16 products: a lane holds half of the scores of one query row.
+#pragma once
+#include "attn_dev.hpp"
+
+namespace ember_attn_impl {
+
+constexpr int kWideThreads = 256, kWideRows = 128;
+
+template <bool BF16>
+__device__ inline f16v mma32(s8 a, s8 b, f16v c) {
+  if constexpr (BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <int DP>
+struct WideLds {
+  static constexpr int kKeys = DP <= 128 ? 64 : 32;  // per tile
+  static constexpr int kCH = DP / 8;                 // 16-byte chunks of a row
+  static constexpr int kTile = kKeys * kCH * 16;
+  static constexpr int kStage = 2 * kTile;           // K and V
+  static constexpr int kBytes = 2 * kStage;
+};
+
+// The sequence of row i of the batch, n_seqs for rows of none.
+__device__ inline int seq_of(const CacheArgs& c, int i) {
+  if (!c.q_start) return i;
+  int lo = 0, hi = c.n_seqs;  // the first b with q_start[b + 1] > i
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (c.q_start[mid + 1] > i) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+// SHARED: the rows are those of the whole batch, the keys the first `end` of sequence 0's. Otherwise blockIdx.y is the sequence, and
+// keys before `begin` are left out.
+template <int T, int IO, int DP, bool GEN, bool SHARED>
+__global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a, Parts parts, int part0, int tiles, int splits,
+                                                                                 int chunk, int begin, int end) {
+  using O = Op<T>;
+  using L = WideLds<DP>;
+  constexpr int CH = L::kCH, KT = L::kKeys, NL = KT * CH / kWideThreads, KS = DP / 16, DT = DP / 32, NS = KT / 32;
+  constexpr int RPI = kWideThreads / CH;  // rows of a tile that one load of all threads covers
+  extern __shared__ __attribute__((aligned(256))) char lds[];
+  __shared__ int bounds[4][4];
+  const CacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, n32 = lane & 31;
+  // the block: KV head fastest (of 8, each stays on one XCD, whose L2 then holds its keys for all row tiles), the last rows, which
+  // see the most keys, first
+  int x = blockIdx.x;
+  const int kvh = x % c.n_kv;
+  x /= c.n_kv;
+  const int split = x % splits, r0 = (tiles - 1 - x / splits) * kWideRows;
+  const int kv_seq = SHARED ? 0 : blockIdx.y;
+  int first = 0, count = c.n_tokens, len = 0, prefix = 0;
+  int64_t p0 = 0;
+  if constexpr (!SHARED) {
+    seq_rows(c, kv_seq, first, count);
+    len = seq_len(c, kv_seq);
+    p0 = (int64_t)len - (c.q_start ? c.q_start[kv_seq + 1] - first : 1);
+    count = min(count, c.max_q);
+    prefix = a.prefix ? a.prefix[kv_seq] : 0;
+    if (r0 >= count * a.G) return;
+  }
+  // this lane's query row
+  const int r = r0 + wave * 32 + n32, tok = r / a.G, h = kvh * a.G + (r - tok * a.G);
+  bool ok = r < count * a.G;
+  int64_t p = p0 + tok;
+  if constexpr (SHARED) {
+    int b = ok ? seq_of(c, tok) : c.n_seqs;
+    ok = b < c.n_seqs;
+    b = ok ? b : 0;
+    int f, n;
+    seq_rows(c, b, f, n);
+    ok = ok && tok >= f && tok - f < min(n, c.max_q);
+    len = seq_len(c, b);
+    p = (int64_t)len - (c.q_start ? c.q_start[b + 1] - f : 1) + (tok - f);
+    prefix = a.prefix ? a.prefix[b] : 0;
+  }
+  Span see = visible(a, p, len, prefix);
+  see.lo = max(see.lo, begin);
+  if constexpr (SHARED) see.hi = min(see.hi, end);
+  const bool blind = !ok || see.lo >= see.hi;
+  // keys that any row of the wave sees, of the block; and that all rows of the wave see
+  int w_lo = blind ? INT32_MAX : see.lo, w_hi = blind ? 0 : see.hi, all_lo = ok ? see.lo : 0, all_hi = ok ? see.hi : INT32_MAX;
+  for (int k = 16; k; k >>= 1) {
+    w_lo = min(w_lo, __shfl_xor(w_lo, k));
+    w_hi = max(w_hi, __shfl_xor(w_hi, k));
+    all_lo = max(all_lo, __shfl_xor(all_lo, k));
+    all_hi = min(all_hi, __shfl_xor(all_hi, k));
+  }
+  w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+  w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  if (lane == 0) {
+    bounds[wave][0] = w_lo;
+    bounds[wave][1] = w_hi;
+    bounds[wave][2] = all_lo;
+    bounds[wave][3] = all_hi;
+  }
+  __syncthreads();
+  const int lo = min(min(bounds[0][0], bounds[1][0]), min(bounds[2][0], bounds[3][0]));
+  const int hi = max(max(bounds[0][1], bounds[1][1]), max(bounds[2][1], bounds[3][1]));
+  const int b_lo = max(max(bounds[0][2], bounds[1][2]), max(bounds[2][2], bounds[3][2]));
+  const int b_hi = min(min(bounds[0][3], bounds[1][3]), min(bounds[2][3], bounds[3][3]));
+  // (lo is INT32_MAX and hi 0 where no row sees a key: no tiles)
+  const int64_t k0l = hi ? (int64_t)(lo & ~(KT - 1)) + (int64_t)split * chunk : 0;
+  const int k0 = (int)min(k0l, (int64_t)hi), k1 = (int)min((int64_t)hi, k0l + chunk);
+
+  // the query row as B operand
+  s8 qf[KS];
+  float mul = a.scale * (GEN && a.softcap > 0.0f ? 2.0f / a.softcap : 1.0f) * kLog2e;
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (ok ? (int64_t)(first + tok) * a.q_stride + (int64_t)h * c.D : 0);
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * half;
+      qf[s] = s8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (ok && d < c.D) qf[s] = *reinterpret_cast<const s8*>(q + d);
+      if constexpr (IO == EMBER_TYPE_BF16 && !O::kBf16)
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(ember_moe::bf16_f32((uint16_t)qf[s][i])));
+    }
+    if constexpr (IO == EMBER_TYPE_BF16 && !O::kBf16) {
+      // (as in attn_step_kernel: bf16 rows as fp16, scaled by a power of two)
+      top = max_lanes32(top);
+      int e = 0;
+      if (top > 0.0f && top <= 3.4028235e38f) (void)__builtin_frexpf(top, &e);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        h8 y;
+        for (int i = 0; i < 8; ++i) y[i] = (_Float16)__builtin_ldexpf(ember_moe::bf16_f32((uint16_t)qf[s][i]), -e);
+        qf[s] = __builtin_bit_cast(s8, y);
+      }
+      mul = fminf(__builtin_ldexpf(mul, e), 3e38f);
+    }
+  }
+  const Scores sc{mul, GEN && a.softcap > 0.0f ? a.softcap * kLog2e : 0.0f, GEN && a.slopes && ok ? a.slopes[h] * kLog2e : 0.0f};
+  const int pos = (int)p;
+  if (!ok) see = {0, INT32_MAX};
+
+  f16v o[DT];
+  float m = kNoScore, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+
+  // loads: row tid / CH (+ RPI i) of a tile, chunk tid % CH: 8 values, 16 bytes of halves or 8 codes
+  const int l_row = tid / CH, l_ch = tid % CH;
+  const bool l_in = l_ch * 8 < c.D;
+  const bool whole = !c.pages || c.page.d % KT == 0;  // a tile lies in one page
+  u4 kr[NL], vr[NL];
+  uint32_t ks_[NL], vs_[NL];  // Q8_0: the scales' bits
+  uint32_t torn = 0;          // bit i: this thread's row i is in no page
+  auto load = [&](int kt) {
+    uint32_t base = 0;
+    if (whole) {
+      const int64_t rr = cache_row(c, kv_seq, kt);
+      base = rr < 0 ? ~0u : (uint32_t)(rr + (int64_t)kvh * c.page.d);
+    }
+    torn = 0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int j = min(kt + l_row + i * RPI, hi - 1);
+      uint32_t row;
+      if (whole) {
+        row = base == ~0u ? ~0u : base + (uint32_t)(j - kt);
+      } else {
+        const int64_t rr = cache_row(c, kv_seq, j);
+        row = rr < 0 ? ~0u : (uint32_t)(rr + (int64_t)kvh * c.page.d);
+      }
+      if (row == ~0u) {
+        torn |= 1u << i;
+        row = 0;
+      }
+      const int64_t at = ((int64_t)row * c.D + l_ch * 8) * O::kBytes;
+      kr[i] = vr[i] = u4{0, 0, 0, 0};
+      ks_[i] = vs_[i] = 0;
+      if (l_in) {
+        if constexpr (O::kQ8) {
+          const u2 kk = *reinterpret_cast<const u2*>(static_cast<const char*>(c.k) + at), vv = *reinterpret_cast<const u2*>(static_cast<const char*>(c.v) + at);
+          kr[i] = u4{kk[0], kk[1], 0, 0};
+          vr[i] = u4{vv[0], vv[1], 0, 0};
+          const int64_t sat = (int64_t)row * (c.D / 32) + l_ch / 4;
+          ks_[i] = __builtin_bit_cast(uint16_t, c.ks[sat]);
+          vs_[i] = __builtin_bit_cast(uint16_t, c.vs[sat]);
+        } else {
+          kr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.k) + at);
+          vr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.v) + at);
+        }
+      }
+    }
+  };
+  // into stage s; values of keys that the block does not see as zeros; whether one in this thread's is not finite
+  auto store = [&](int kt, int s) -> bool {
+    char* const kl = lds + s * L::kStage;
+    char* const vl = kl + L::kTile;
+    const bool inside = kt >= lo && kt + KT <= hi;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int key = l_row + i * RPI;
+      u4 kk = kr[i], vv = vr[i];
+      if constexpr (O::kQ8) {
+        auto held = [](u4 w, uint32_t bits) {
+          const _Float16 s_ = __builtin_bit_cast(_Float16, (uint16_t)bits);
+          return __builtin_bit_cast(u4, codes_times(u2{w[0], w[1]}, h8{s_, s_, s_, s_, s_, s_, s_, s_}));
+        };
+        kk = held(kk, ks_[i]);
+        vv = held(vv, vs_[i]);
+      }
+      if (!inside && (kt + key < lo || kt + key >= hi)) vv = u4{0, 0, 0, 0};
+      // a key in no page: NaN, which makes its scores so
+      if (torn >> i & 1) kk = u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+      *reinterpret_cast<u4*>(kl + k_at<CH>(key, l_ch)) = kk;
+      *reinterpret_cast<u4*>(vl + v_at<CH, false>(key, l_ch)) = vv;
+      constexpr uint32_t e = O::kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) odd |= (vv[w] & e) == e || (vv[w] & (e << 16)) == (e << 16);
+    }
+    return odd;
+  };
+  // all waves past the stage's last readers, and its writers done; whether the tile needs the careful sum
+  auto meet = [&](int kt, bool odd) -> bool {
+    if (kt < b_lo || kt + KT > b_hi) return __syncthreads_or(odd) != 0;
+    __syncthreads();
+    return false;
+  };
+
+  bool careful = false;
+  if (k0 < k1) {
+    load(k0);
+    const bool odd = store(k0, 0);
+    careful = meet(k0, odd);
+  }
+  for (int kt = k0, st = 0; kt < k1; kt += KT, st ^= 1) {
+    const bool more = kt + KT < k1;
+    if (more) load(kt + KT);
+    if (kt < w_hi && kt + KT > w_lo) {
+      const char* const kl = lds + st * L::kStage;
+      const char* const vl = kl + L::kTile;
+      f16v s[NS];
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < KS; ++q) {
+          const s8 kf = *reinterpret_cast<const s8*>(kl + k_at<CH>(u * 32 + n32, 2 * q + half));
+          s[u] = mma32<O::kBf16>(kf, qf[q], s[u]);
+        }
+      }
+      // key of score i of half-tile u: 8 (i / 4) + 4 half + i % 4
+      const bool masked = kt < all_lo || kt + KT > all_hi;
+      if (GEN) {
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[u][i] = sc(s[u][i], kt + u * 32 + 8 * (i >> 2) + 4 * half + (i & 3) - pos);
+      }
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = kt + u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+            if (key < see.lo || key >= see.hi) s[u][i] = -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+      top = max_lanes32(top);
+      const float mc = GEN ? 1.0f : mul;
+      top *= mc;
+      if (__ballot(top > m + 8.0f)) {  // (as in attn_step_kernel)
+        const float m2 = fmaxf(m, top), al = exp2_fast(m - m2);
+        m = m2;
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          for (int i = 0; i < 16; ++i) o[d][i] *= al;
+      }
+      s8 pf[NS * 2];
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = exp2_fast(__builtin_fmaf(s[u][i], mc, -m));
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) l += (s[u][i] + s[u][i + 1]) + (s[u][i + 2] + s[u][i + 3]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          pf[u * 2 + q] = __builtin_bit_cast(s8, u4{pack2<O::kBf16>(s[u][8 * q], s[u][8 * q + 1]), pack2<O::kBf16>(s[u][8 * q + 2], s[u][8 * q + 3]),
+                                                    pack2<O::kBf16>(s[u][8 * q + 4], s[u][8 * q + 5]), pack2<O::kBf16>(s[u][8 * q + 6], s[u][8 * q + 7])});
+      }
+      // V^T: columns 32 d + lane % 32, the keys of score order: 16 q + 4 half + 0 .. 3, and 8 further
+      const int v_key = 4 * half + ((lane & 15) >> 2), v_c = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+      auto v_frag = [&](int d, int q) -> s8 {
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + v_key, 4 * d + v_c) + (lane & 1) * 8));
+        const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + 8 + v_key, 4 * d + v_c) + (lane & 1) * 8));
+        return s8{y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
+      };
+      if (careful && masked) {
+        // (as in attn_step_kernel: values that are not finite, among keys that some rows see and others do not)
+        const short one = O::kBf16 ? (short)0x3f80 : (short)0x3c00, ex = O::kBf16 ? (short)0x7f80 : (short)0x7c00;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          f16v hit;
+          for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < NS * 2; ++q) {
+            const s8 v = v_frag(d, q);
+            s8 flag, fine, vis;
+            for (int i = 0; i < 8; ++i) {
+              const bool f = (v[i] & ex) == ex;
+              flag[i] = f ? one : (short)0;
+              fine[i] = f ? (short)0 : v[i];
+              const int key = kt + 16 * q + 8 * (i >> 2) + 4 * half + (i & 3);
+              vis[i] = key >= see.lo && key < see.hi ? one : (short)0;
+            }
+            hit = mma32<O::kBf16>(flag, vis, hit);
+            o[d] = mma32<O::kBf16>(fine, pf[q], o[d]);
+          }
+          for (int i = 0; i < 16; ++i)
+            if (hit[i] > 0.0f) o[d][i] = __builtin_nanf("");
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < NS * 2; ++q)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[d] = mma32<O::kBf16>(v_frag(d, q), pf[q], o[d]);
+      }
+    }
+    if (more) {
+      const bool odd = store(kt + KT, st ^ 1);
+      careful = meet(kt + KT, odd);
+    }
+  }
+
+  if (!ok) return;  // (no barrier follows)
+  l = sum_lanes32(l);
+  // column 32 d + 8 (i / 4) + 4 half + i % 4 of this lane's row
+  if (parts.o) {
+    const int64_t row = (int64_t)(part0 + split) * parts.rows + (int64_t)(first + tok) * a.H + h;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      for (int i = 0; i < 16; i += 4) {
+        const int col = d * 32 + 2 * i + 4 * half;
+        if (col < c.D) *reinterpret_cast<f4*>(parts.o + row * c.D + col) = f4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+      }
+    if (half == 0) {
+      parts.ml[row * 2] = m;
+      parts.ml[row * 2 + 1] = l;
+    }
+  } else {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      for (int i = 0; i < 16; i += 4) {
+        const int col = d * 32 + 2 * i + 4 * half;
+        const u2 y = {pack2<IO == EMBER_TYPE_BF16>(o[d][i] * inv, o[d][i + 1] * inv), pack2<IO == EMBER_TYPE_BF16>(o[d][i + 2] * inv, o[d][i + 3] * inv)};
+        if (col < c.D) *reinterpret_cast<u2*>(out + col) = y;
+      }
+  }
+}
+
+template <int T, int IO, int DP, bool SHARED>
+int launch_wide(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st) {
+  const int64_t rows = (int64_t)(SHARED ? a.c.n_tokens : a.c.max_q) * a.G, tiles = (rows + kWideRows - 1) / kWideRows;
+  if (tiles * w.splits * a.c.n_kv > 0x7fffffff) return EMBER_ERR_SHAPE;
+  const dim3 grid((unsigned)(tiles * w.splits * a.c.n_kv), SHARED ? 1 : a.c.n_seqs);
+  constexpr size_t lds = WideLds<DP>::kBytes;
+  static_assert(lds <= 65536, "no attribute needed");
+  if (a.softcap > 0.0f || a.slopes)
+    attn_wide_kernel<T, IO, DP, true, SHARED><<<grid, kWideThreads, lds, st>>>(a, p, w.part0, (int)tiles, w.splits, w.chunk, w.begin, w.end);
+  else
+    attn_wide_kernel<T, IO, DP, false, SHARED><<<grid, kWideThreads, lds, st>>>(a, p, w.part0, (int)tiles, w.splits, w.chunk, w.begin, w.end);
+  return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
+}
+
+template <int T, int IO>
+int launch_wide_type(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st) {
+  if (w.end) {  // the shared pages
+    if (a.c.D <= 64) return launch_wide<T, IO, 64, true>(a, p, w, st);
+    if (a.c.D <= 128) return launch_wide<T, IO, 128, true>(a, p, w, st);
+    return launch_wide<T, IO, 256, true>(a, p, w, st);
+  }
+  if (a.c.D <= 64) return launch_wide<T, IO, 64, false>(a, p, w, st);
+  if (a.c.D <= 128) return launch_wide<T, IO, 128, false>(a, p, w, st);
+  return launch_wide<T, IO, 256, false>(a, p, w, st);
+}
+
+}  // namespace ember_attn_impl
