@@ -67,6 +67,16 @@ __device__ inline s8 codes_times(u2 w, h8 s) {
   return __builtin_bit_cast(s8, __builtin_bit_cast(h8, c) * s);
 }
 
+// Whether one of 8 halves is infinite or NaN.
+template <bool BF16>
+__device__ inline bool not_finite(u4 v) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  bool r = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) r |= (v[w] & e) == e || (v[w] & (e << 16)) == (e << 16);
+  return r;
+}
+
 // Largest value over the lanes that hold the same query row.
 __device__ inline float max_lanes32(float x) {  // lanes l, l ^ 32
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

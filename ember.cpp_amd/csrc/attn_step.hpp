@@ -152,21 +152,24 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
     rows_next = look_up(kt + kStepWaves * kTile);
   }
   for (; kt < k1; kt += kStepWaves * kTile) {
-    // values of keys outside the rows' span count for none of them, whatever they hold
+    // values of keys outside the rows' span count for none of them, whatever they hold: stored as zeros. So are, in a tile that
+    // some rows see in part only, values that are not finite (a weight of 0 times one is NaN), and their keys are noted
     const bool inside = kt >= lo && kt + kTile <= hi;
-    bool odd = false;  // a value in this lane that is not finite
+    const bool masked = kt < all_lo || kt + kTile > all_hi || !inside, part = masked && pa != pz;
+    uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
       *reinterpret_cast<u4*>(kt_ + k_at<CH>(key, cc)) = reg.k[i];
       u4 v = reg.v[i];
       if (!inside && (kt + key < lo || kt + key >= hi)) v = u4{0, 0, 0, 0};
-      *reinterpret_cast<u4*>(vt_ + v_at<CH, O::kQ8>(key, cc)) = v;
       if constexpr (!O::kQ8) {
-        constexpr uint32_t e = O::kBf16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd |= (v[w] & e) == e || (v[w] & (e << 16)) == (e << 16);
+        if (part && not_finite<O::kBf16>(v)) {
+          v = u4{0, 0, 0, 0};
+          odd |= 1u << key;
+        }
       }
+      *reinterpret_cast<u4*>(vt_ + v_at<CH, O::kQ8>(key, cc)) = v;
     }
     h8 k_scale[2];
     if constexpr (O::kQ8) {
@@ -176,9 +179,12 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
         const bool out = kt + lane < lo || kt + lane >= hi;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          const _Float16 sc = out ? (_Float16)0.0f : x.h[i];
+          _Float16 sc = out ? (_Float16)0.0f : x.h[i];
+          if (part && (__builtin_bit_cast(uint16_t, sc) & 0x7c00u) == 0x7c00u) {
+            sc = (_Float16)0.0f;
+            odd |= 1u << lane;
+          }
           vs_[i * kTile + lane] = sc;
-          odd |= (__builtin_bit_cast(uint16_t, sc) & 0x7c00u) == 0x7c00u;
         }
       }
       k_scale[0] = __builtin_bit_cast(h8, reg.ks[0]);
@@ -215,7 +221,6 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
       }
     }
 
-    const bool masked = kt < all_lo || kt + kTile > all_hi || kt < lo || kt + kTile > hi;
     const bool torn = __ballot(here == ~0u) != 0;  // keys in no page: their scores are NaN
     uint32_t bad = 0;
     if (torn) bad = (uint32_t)__ballot(here == ~0u);
@@ -262,32 +267,12 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
         return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       }
     };
-    if (masked && pa != pz && __ballot(odd)) {
-      // a value that is not finite among keys that some rows see and others do not (their weight 0 times it were NaN): it
-      // counts as 0 in the sum, and the rows that see it get NaN in its column
-      const short one = O::kBf16 ? (short)0x3f80 : (short)0x3c00, ex = O::kBf16 ? (short)0x7f80 : (short)0x7c00;
-      s8 vis;
-      for (int i = 0; i < 8; ++i) {
-        const int key = kt + (i >> 2) * 16 + g * 4 + (i & 3);
-        vis[i] = key >= max(see.lo, lo) && key < min(see.hi, hi) ? one : (short)0;
-      }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const s8 v = v_frag(d);
-        s8 flag, fine;
-        for (int i = 0; i < 8; ++i) {
-          const bool f = (v[i] & ex) == ex;
-          flag[i] = f ? one : (short)0;
-          fine[i] = f ? (short)0 : v[i];
-        }
-        const f4 hit = mma16<O::kBf16>(flag, vis, f4{0, 0, 0, 0});
-        o[d] = mma16<O::kBf16>(fine, pf, o[d]);
-        for (int i = 0; i < 4; ++i)
-          if (hit[i] > 0.0f) o[d][i] = __builtin_nanf("");
-      }
-    } else {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = mma16<O::kBf16>(v_frag(d), pf, o[d]);
+    for (int d = 0; d < DT; ++d) o[d] = mma16<O::kBf16>(v_frag(d), pf, o[d]);
+    if (part && __ballot(odd != 0)) {  // a row that sees one of those keys: NaN by its sum of weights
+      for (int k = 32; k; k >>= 1) odd |= __shfl_xor(odd, k);
+      const int from = max(max(see.lo, lo) - kt, 0), to = min(min(see.hi, hi) - kt, kTile);
+      if (from < to && (odd >> from & (~0u >> (32 - (to - from))))) l = __builtin_nanf("");
     }
   }
 

@@ -50,6 +50,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
   constexpr int RPI = kWideThreads / CH;  // rows of a tile that one load of all threads covers
   extern __shared__ __attribute__((aligned(256))) char lds[];
   __shared__ int bounds[4][4];
+  __shared__ unsigned long long odd_keys[4];  // of tile n at n % 4: its keys whose values are not all finite
   const CacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, n32 = lane & 31;
   // the block: KV head fastest (of 8, each stays on one XCD, whose L2 then holds its keys for all row tiles), the last rows, which
@@ -106,6 +107,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
     bounds[wave][2] = all_lo;
     bounds[wave][3] = all_hi;
   }
+  if (tid < 4) odd_keys[tid] = 0;
   __syncthreads();
   const int lo = min(min(bounds[0][0], bounds[1][0]), min(bounds[2][0], bounds[3][0]));
   const int hi = max(max(bounds[0][1], bounds[1][1]), max(bounds[2][1], bounds[3][1]));
@@ -199,12 +201,12 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
       }
     }
   };
-  // into stage s; values of keys that the block does not see as zeros; whether one in this thread's is not finite
-  auto store = [&](int kt, int s) -> bool {
+  // into stage s; values of keys that the block does not see as zeros. A tile that some rows see in part only (`part`) must not
+  // hold values that are not finite, since a weight of 0 times one is NaN: they are stored as zeros too, and their key is noted
+  auto store = [&](int kt, int s, bool part, unsigned long long* odd) {
     char* const kl = lds + s * L::kStage;
     char* const vl = kl + L::kTile;
     const bool inside = kt >= lo && kt + KT <= hi;
-    bool odd = false;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int key = l_row + i * RPI;
@@ -220,32 +222,27 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
       if (!inside && (kt + key < lo || kt + key >= hi)) vv = u4{0, 0, 0, 0};
       // a key in no page: NaN, which makes its scores so
       if (torn >> i & 1) kk = u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+      if (part && not_finite<O::kBf16>(vv)) {
+        vv = u4{0, 0, 0, 0};
+        atomicOr(odd, 1ull << key);
+      }
       *reinterpret_cast<u4*>(kl + k_at<CH>(key, l_ch)) = kk;
       *reinterpret_cast<u4*>(vl + v_at<CH, false>(key, l_ch)) = vv;
-      constexpr uint32_t e = O::kBf16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) odd |= (vv[w] & e) == e || (vv[w] & (e << 16)) == (e << 16);
     }
-    return odd;
   };
-  // all waves past the stage's last readers, and its writers done; whether the tile needs the careful sum
-  auto meet = [&](int kt, bool odd) -> bool {
-    if (kt < b_lo || kt + KT > b_hi) return __syncthreads_or(odd) != 0;
-    __syncthreads();
-    return false;
-  };
+  auto in_part = [&](int kt) { return kt < b_lo || kt + KT > b_hi; };
 
-  bool careful = false;
   if (k0 < k1) {
     load(k0);
-    const bool odd = store(k0, 0);
-    careful = meet(k0, odd);
+    store(k0, 0, in_part(k0), &odd_keys[0]);
+    __syncthreads();
   }
-  for (int kt = k0, st = 0; kt < k1; kt += KT, st ^= 1) {
+  for (int kt = k0, n = 0; kt < k1; kt += KT, ++n) {
     const bool more = kt + KT < k1;
     if (more) load(kt + KT);
+    if (tid == 0) odd_keys[(n + 2) & 3] = 0;  // (two barriers after it was read, one before it is written again)
     if (kt < w_hi && kt + KT > w_lo) {
-      const char* const kl = lds + st * L::kStage;
+      const char* const kl = lds + (n & 1) * L::kStage;
       const char* const vl = kl + L::kTile;
       f16v s[NS];
 #pragma unroll
@@ -273,6 +270,10 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
             const int key = kt + u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
             if (key < see.lo || key >= see.hi) s[u][i] = -INFINITY;
           }
+        if (const uint64_t odd = odd_keys[n & 3]) {  // a row that sees one of them: NaN by its sum of weights
+          const int from = max(see.lo - kt, 0), to = min(see.hi - kt, KT);
+          if (from < to && (odd >> from & (~0ull >> (64 - (to - from))))) l = __builtin_nanf("");
+        }
       }
       float top = s[0][0];
 #pragma unroll
@@ -304,46 +305,17 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
       }
       // V^T: columns 32 d + lane % 32, the keys of score order: 16 q + 4 half + 0 .. 3, and 8 further
       const int v_key = 4 * half + ((lane & 15) >> 2), v_c = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-      auto v_frag = [&](int d, int q) -> s8 {
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + v_key, 4 * d + v_c) + (lane & 1) * 8));
-        const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + 8 + v_key, 4 * d + v_c) + (lane & 1) * 8));
-        return s8{y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
-      };
-      if (careful && masked) {
-        // (as in attn_step_kernel: values that are not finite, among keys that some rows see and others do not)
-        const short one = O::kBf16 ? (short)0x3f80 : (short)0x3c00, ex = O::kBf16 ? (short)0x7f80 : (short)0x7c00;
+#pragma unroll
+      for (int q = 0; q < NS * 2; ++q)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          f16v hit;
-          for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
-#pragma unroll
-          for (int q = 0; q < NS * 2; ++q) {
-            const s8 v = v_frag(d, q);
-            s8 flag, fine, vis;
-            for (int i = 0; i < 8; ++i) {
-              const bool f = (v[i] & ex) == ex;
-              flag[i] = f ? one : (short)0;
-              fine[i] = f ? (short)0 : v[i];
-              const int key = kt + 16 * q + 8 * (i >> 2) + 4 * half + (i & 3);
-              vis[i] = key >= see.lo && key < see.hi ? one : (short)0;
-            }
-            hit = mma32<O::kBf16>(flag, vis, hit);
-            o[d] = mma32<O::kBf16>(fine, pf[q], o[d]);
-          }
-          for (int i = 0; i < 16; ++i)
-            if (hit[i] > 0.0f) o[d][i] = __builtin_nanf("");
+          const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + v_key, 4 * d + v_c) + (lane & 1) * 8));
+          const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + 8 + v_key, 4 * d + v_c) + (lane & 1) * 8));
+          o[d] = mma32<O::kBf16>(s8{y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]}, pf[q], o[d]);
         }
-      } else {
-#pragma unroll
-        for (int q = 0; q < NS * 2; ++q)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[d] = mma32<O::kBf16>(v_frag(d, q), pf[q], o[d]);
-      }
     }
-    if (more) {
-      const bool odd = store(kt + KT, st ^ 1);
-      careful = meet(kt + KT, odd);
-    }
+    if (more) store(kt + KT, (n + 1) & 1, in_part(kt + KT), &odd_keys[(n + 1) & 3]);
+    __syncthreads();
   }
 
   if (!ok) return;  // (no barrier follows)

@@ -78,7 +78,8 @@ int ember_kv_load(const ember_kv_cache* c, const ember_kv_batch* b, void* k, int
  * (< kv_len[b]) is visible if j <= p or j < prefix[b], and, where window > 0, p - j < window. Its score is
  *   s = scale * (q . k_j);  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s -= slopes[h] * |p - j|
  * and the output row the softmax-weighted sum of the visible keys' values, zeros if no key is visible. Keys and
- * values that a row does not see have no effect on it, whatever they hold. */
+ * values that a row does not see have no effect on it, whatever they hold; a row that sees one that is infinite or NaN is
+ * not finite in the columns that hold it, or in all. */
 typedef struct ember_attn_opts {
   int n_heads;           /* a multiple of n_kv, up to 128 per KV head */
   float scale;           /* > 0 */
