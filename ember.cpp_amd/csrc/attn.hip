@@ -6,45 +6,78 @@
 namespace ember_attn_impl {
 namespace {
 
-// Rows of parts (Parts) as output rows: a wave per row. Its lanes first hold one part's maximum and sum each, then the row's columns.
+// Rows of parts (Parts) as output rows: a block per row, four waves on a quarter of the parts each. A wave's lanes first hold one
+// part's maximum and sum each, then the row's columns. (A wave alone took 126 us for 32 rows of 256 parts: one load after another.)
 template <int IO>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts) {
+  __shared__ f4 xs[4][64];
+  __shared__ float ms[4], sums[4];
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int tok = at / a.H, h = at - tok * a.H;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.x / a.H, h = blockIdx.x - tok * a.H;
   int first, count;
   seq_rows(c, blockIdx.y, first, count);
   if (tok >= min(count, c.max_q)) return;
   const int64_t row = (int64_t)(first + tok) * a.H + h;
-  float M = kNoScore;
-  for (int p = lane; p < parts.n; p += 64) M = fmaxf(M, parts.ml[(p * parts.rows + row) * 2]);
+  const int per = (parts.n + 3) / 4, from = wave * per, n = min(per, parts.n - from);  // (at most 128 parts a wave)
+  const int d = min(lane * 4, c.D - 4);
+  float m[2] = {kNoScore, kNoScore}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (u * 64 + lane < n) {
+      const float* ml = parts.ml + ((from + u * 64 + lane) * parts.rows + row) * 2;
+      m[u] = ml[0];
+      l[u] = ml[1];
+    }
+  float M = fmaxf(m[0], m[1]);
   for (int k = 32; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
   float sum = 0.0f;
   f4 x = {0, 0, 0, 0};
-  const int d = lane * 4;
-  for (int p0 = 0; p0 < parts.n; p0 += 64) {
-    float w = 0.0f, l = 0.0f;
-    if (p0 + lane < parts.n) {
-      const float* ml = parts.ml + ((p0 + lane) * parts.rows + row) * 2;
-      l = ml[1];
-      w = exp2_fast(ml[0] - M);
-    }
-    sum += l * w;
-    for (uint64_t todo = __ballot(l != 0.0f); todo; todo &= todo - 1) {  // (parts without a visible key hold nothing)
-      const int p = __ffsll((unsigned long long)todo) - 1;
-      const float wp = __shfl(w, p);
-      if (d < c.D) {
-        f4 y = *reinterpret_cast<const f4*>(parts.o + ((p0 + p) * parts.rows + row) * c.D + d);
-        y *= wp;
-        x += y;
+  const float* const o = parts.o + (from * parts.rows + row) * c.D + d;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float w = exp2_fast(m[u] - M);
+    sum += l[u] * w;
+    const float live = l[u] != 0.0f ? w : -1.0f;  // (parts without a visible key hold nothing; NaN is not 0)
+    const int end = min(64, n - u * 64);
+    for (int p0 = 0; p0 < end; p0 += 8) {
+      f4 y[8];
+      float wp[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        wp[i] = __shfl(live, (p0 + i) & 63);
+        y[i] = f4{0, 0, 0, 0};
+        if (p0 + i < end && wp[i] != -1.0f) y[i] = *reinterpret_cast<const f4*>(o + (u * 64 + p0 + i) * parts.rows * c.D);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p0 + i < end && wp[i] != -1.0f) {
+          y[i] *= wp[i];
+          x += y[i];
+        }
     }
   }
   for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+  xs[wave][lane] = x;
+  if (lane == 0) {
+    ms[wave] = M;
+    sums[wave] = sum;
+  }
+  __syncthreads();
+  if (wave || lane * 4 >= c.D) return;
+  M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  sum = 0.0f;
+  x = f4{0, 0, 0, 0};
+  for (int w = 0; w < 4; ++w) {
+    const float al = exp2_fast(ms[w] - M);
+    sum += sums[w] * al;
+    f4 y = xs[w][lane];
+    y *= al;
+    x += y;
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   x *= inv;
   const u2 y = {pack2<IO == EMBER_TYPE_BF16>(x[0], x[1]), pack2<IO == EMBER_TYPE_BF16>(x[2], x[3])};
-  if (d < c.D) *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
+  *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
 }
 
 }  // namespace
@@ -52,20 +85,30 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts)
 AttnPlan attn_plan(const AttnArgs& a) {
   AttnPlan p{};
   const CacheArgs& c = a.c;
-  const int64_t rows = (int64_t)c.max_q * a.G;
+  const bool q8 = c.type == EMBER_TYPE_Q8_0;
+  const int64_t rows = (int64_t)c.max_q * a.G, row_bytes = q8 ? c.D + c.D / 16 : 2 * c.D;
   p.step = rows <= 64;
+  // Shared pages cost a launch and a part more per row, and what they save are reads of the same memory again, which the caches serve
+  // in part: from some 128 MB on (Q8_0, 8 KV heads of 128, shared / not: 32 sequences x 1024 tokens, 71 MB, 30 / 22 us; 4 x 16384, 107 MB,
+  // 35 / 34; 32 x 4096, 276 MB, 33 / 50; 96 x 8192, 1.7 GB, 83 / 221).
   p.begin = std::min(a.shared, c.cap);
+  if ((int64_t)(c.n_seqs - 1) * p.begin * c.n_kv * 2 * row_bytes < (int64_t)1 << 27) p.begin = 0;
+  // `keys` in parts of whole `unit`s, so many that there are about `want` blocks
   auto split = [](int64_t keys, int64_t blocks, int64_t want, int unit, int& splits, int& chunk) {
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>({keys / unit, 256, (want + blocks - 1) / blocks}));
     chunk = (int)((keys + n * unit - 1) / (n * unit)) * unit;
     splits = (int)((keys + chunk - 1) / chunk);
   };
-  // keys that the rows of a sequence can see at most, and one tile for where they begin within one
+  // keys that the rows of a sequence can see at most, and a tile's where they may begin within one
   int64_t range = c.cap - p.begin;
   if (a.window > 0 && !a.prefix) range = std::min<int64_t>(range, (int64_t)a.window + c.max_q - 1);
-  range = std::max<int64_t>(range, 1) + 63;
+  range = std::max<int64_t>(range, 1) + (a.window > 0 || p.begin % 64 ? 63 : 0);
   const int64_t groups = (int64_t)c.n_seqs * c.n_kv;
-  if (p.step) split(range, groups * ((rows + 15) / 16), 2048, 128, p.splits, p.chunk);
+  // Step kernel: one block for each place that 256 CUs have (more parts cost more than they level out: 131000 bf16 tokens on 512 / 1024 /
+  // 2048 blocks 102 / 108 / 116 us, 8 sequences of up to 20000 Q8_0 tokens on 512 / 768 / 1024 78 / 66 / 77); up to 256 keys in one part,
+  // which saves the join (256 keys 9.3 us in one part, 10.7 in two; 512 11.6, 11.0).
+  const int places = 256 * (c.D > 128 ? (q8 ? 2 : 1) : q8 ? 3 : 2);
+  if (p.step) split(range, groups * ((rows + 15) / 16), range <= 256 ? 1 : places, 128, p.splits, p.chunk);
   else split(range, groups * ((rows + 127) / 128), 512, 256, p.splits, p.chunk);
   if (p.begin) split(p.begin, c.n_kv * (((int64_t)c.n_tokens * a.G + 127) / 128), 512, 256, p.shared_splits, p.shared_chunk);
   p.parts = p.splits + p.shared_splits > 1 ? p.splits + p.shared_splits : 0;
@@ -93,7 +136,8 @@ int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st) {
   if (p.step) s = steps[kind](a, parts, p.shared_splits, p.splits, p.chunk, p.begin, st);
   else s = wides[kind](a, parts, WideCall{p.shared_splits, p.splits, p.chunk, p.begin, 0}, st);
   if (s || !p.parts) return s;
-  const dim3 grid((unsigned)(((int64_t)a.c.max_q * a.H + 3) / 4), a.c.n_seqs);
+  if ((int64_t)a.c.max_q * a.H > 0x7fffffff) return EMBER_ERR_SHAPE;
+  const dim3 grid((unsigned)(a.c.max_q * a.H), a.c.n_seqs);
   if (a.type == EMBER_TYPE_BF16) attn_join_kernel<EMBER_TYPE_BF16><<<grid, 256, 0, st>>>(a, parts);
   else attn_join_kernel<EMBER_TYPE_F16><<<grid, 256, 0, st>>>(a, parts);
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;

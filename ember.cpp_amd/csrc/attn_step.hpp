@@ -3,46 +3,75 @@
 //
 // Bound by the cache's bytes: every key and value is read once, for all heads that share it. A block takes one KV head of one
 // sequence (and one part of its keys, where sequences are few or long: the parts are joined by attn_join_kernel), its four
-// waves take tiles of 32 keys in turn, each on its own: no barrier until the waves' results are joined at the end. A tile's
-// rows are loaded in whole rows into registers while the tile before it is computed, and pass through LDS, which K leaves as
-// the matrix cores' A operand and V transposed. 16 query rows fill an operand's columns; with 4 heads per KV head three quarters
-// of it are idle, which costs nothing while the loads take longer. More rows than 16 are tiles of their own, which read the cache again.
+// waves take tiles of 32 or 64 keys in turn, each on its own: no barrier until the waves' results are joined at the end. A tile
+// passes through LDS, which K leaves as the matrix cores' A operand and V transposed: rows of halves by way of registers, loaded while
+// the tile before is computed (two blocks per CU, some 100 KB of loads on the way: 131000 bf16 tokens, 537 MB, in 102 us, 5.2 TB/s,
+// what a copy reaches); codes straight into LDS, which leaves registers for three blocks per CU, whose waves take turns
+// (48 sequences of 6000 tokens, 627 MB, in 127 us, 4.9 TB/s; by way of registers, two blocks, 145). 16 query rows fill an operand's
+// columns; with 4 heads per KV head three quarters of it are idle, which costs nothing while the loads take longer. More
+// rows than 16 are tiles of their own, which read the cache again.
 #pragma once
 #include "attn_dev.hpp"
 
 namespace ember_attn_impl {
 
-constexpr int kStepThreads = 256, kStepWaves = 4, kTile = 32;
+constexpr int kStepThreads = 256, kStepWaves = 4;
 
 template <int T, int DP>
 struct StepLds {
-  static constexpr int kCH = DP * Op<T>::kBytes / 16;
-  static constexpr int kTileBytes = kTile * kCH * 16;
-  static constexpr int kScaleBytes = Op<T>::kQ8 ? (DP / 32) * kTile * 2 : 0;
+  static constexpr int kKeys = DP <= 64 ? 64 : 32;
+  static constexpr int kCH = DP * Op<T>::kBytes / 16;  // 16-byte chunks of a row
+  static constexpr int kTileBytes = kKeys * kCH * 16;
+  static constexpr int kScaleBytes = Op<T>::kQ8 ? 2 * (DP / 32) * kKeys * 2 : 0;  // of K by key, of V by block
   static constexpr int kWave = 2 * kTileBytes + kScaleBytes;
   static constexpr int kJoin = 16 * DP * 4;  // a wave's result
   static constexpr int kPerWave = kWave > kJoin ? kWave : kJoin;
   static constexpr int kBytes = kStepWaves * kPerWave;
 };
 
-// A wave's loads of one tile: rows of K and V, in order, 16 bytes a lane.
-template <int T, int DP>
-struct TileRegs {
-  static constexpr int kCH = DP * Op<T>::kBytes / 16, kN = kCH / 2;
-  u4 k[kN], v[kN];
-  u4 ks[2];        // Q8_0: the scales of this lane's two keys (l % 16, 16 + l % 16), for K
-  u4 vs;           // and of key l % 32, for V
-};
+// The scales of a Q8_0 row: KS of them if EXACT, otherwise nb and zeros.
+template <int KS>
+using RowScales __attribute__((ext_vector_type(KS))) = _Float16;
+template <int KS, bool EXACT>
+__device__ inline RowScales<KS> row_scales(const _Float16* p, uint32_t row, int nb) {
+  row = row == ~0u ? 0 : row;
+  if constexpr (EXACT) {
+    return *reinterpret_cast<const RowScales<KS>*>(p + (int64_t)row * KS);
+  } else {
+    RowScales<KS> r;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) r[i] = i < nb ? p[(int64_t)row * nb + i] : (_Float16)0.0f;
+    return r;
+  }
+}
 
-template <int T, int IO, int DP, bool GEN>
-__global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_kernel(AttnArgs a, Parts parts, int part0, int tiles, int chunk, int begin) {
+// 16 bytes per lane from global memory into LDS, lane after lane from `lds` on, without registers.
+__device__ inline void load_to_lds(const void* g, char* lds) {
+  __builtin_amdgcn_global_load_lds(g, (EMBER_LDS(void)*)lds, 16, 0, 0);
+}
+// All of this wave's loads, to registers and to LDS, have arrived; all its LDS reads are done.
+__device__ inline void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+__device__ inline void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// EXACT: rows of DP columns, not fewer.
+template <int T, int IO, int DP, bool GEN, bool EXACT>
+__global__ __launch_bounds__(kStepThreads, DP > 128 ? (Op<T>::kQ8 ? 2 : 1) : Op<T>::kQ8 ? 3 : 2) void attn_step_kernel(AttnArgs a, Parts parts, int part0, int tiles, int chunk, int begin) {
   using O = Op<T>;
   using L = StepLds<T, DP>;
-  constexpr int CH = L::kCH, NL = CH / 2, KS = DP / 32, DT = DP / 16;
+  constexpr int KT = L::kKeys, CH = L::kCH, NL = KT * CH / 64, KS = DP / 32, DT = DP / 16, NT = KT / 16;
   extern __shared__ __attribute__((aligned(256))) char lds[];
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n16 = lane & 15;
-  const int split = blockIdx.x / tiles, r0 = (blockIdx.x - split * tiles) * 16, kvh = blockIdx.y, b = blockIdx.z;
+  // (splits slowest: the last ones are empty for short sequences, and were they neighbours, whole XCDs would be: blocks go to these in turn)
+  const int kvh = blockIdx.x, b = blockIdx.y, split = blockIdx.z / tiles, r0 = (blockIdx.z - split * tiles) * 16;
   int first, count;
   seq_rows(c, b, first, count);
   const int nrows = min(16, min(count, c.max_q) * a.G - r0);  // rows of this tile: r0 + n is head n % G of token n / G
@@ -55,7 +84,7 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
   const Span sa = visible(a, pa, len, prefix), sz = visible(a, pz, len, prefix);
   const int lo = max(visible(a, max(pa, (int64_t)0), len, prefix).lo, begin), hi = sz.hi;
   const int all_lo = sz.lo, all_hi = sa.hi;  // (none where the first row is before the first position)
-  const int k0 = (lo & ~(kTile - 1)) + split * chunk, k1 = min(hi, k0 + chunk);
+  const int k0 = (lo & ~(KT - 1)) + split * chunk, k1 = min(hi, k0 + chunk);
 
   // the query rows as B operands: column n16, and for step s the columns of d that K's operand holds in this lane
   s8 qf[KS];
@@ -105,137 +134,167 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
   char* const kt_ = lds + wave * L::kPerWave;
   char* const vt_ = kt_ + L::kTileBytes;
   _Float16* const vs_ = reinterpret_cast<_Float16*>(vt_ + L::kTileBytes);
+  RowScales<KS>* const ks_ = reinterpret_cast<RowScales<KS>*>(vs_ + KS * KT);
   const int ch = c.D * O::kBytes / 16;  // chunks of a row (CH with columns past D, which are zero)
 
-  // cache row (kvh's) of key kt + lane % 32, clamped into the sequence; ~0: in no page
+  // cache row (kvh's) of key kt + lane % KT, clamped into the sequence; ~0: in no page
   auto look_up = [&](int kt) -> uint32_t {
-    const int j = min(kt + (lane & 31), hi - 1);
+    const int j = min(kt + (lane & (KT - 1)), hi - 1);
     const int64_t r = cache_row(c, b, j);
     return r < 0 ? ~0u : (uint32_t)(r + (int64_t)kvh * c.page.d);
   };
-  TileRegs<T, DP> reg;
+  // a tile's rows, in order, 16 bytes a lane: halves by way of registers, since values may have to be put out; codes straight into LDS,
+  // where lane l's 16 bytes come to lie at 16 l: it fetches the chunk that belongs there (k_at, v_at). Of Q8_0 the scales of key lane %
+  // KT as well, in registers: what is put out there is a value's scale
+  u4 kr[O::kQ8 ? 1 : NL], vr[O::kQ8 ? 1 : NL];
+  RowScales<KS> ksc, vsc;
+  auto row_of = [&](uint32_t rows, int key) {
+    const uint32_t row = __shfl(rows, key);
+    return (int64_t)(row == ~0u ? 0 : row) * c.D * O::kBytes;
+  };
   auto load = [&](uint32_t rows) {
+    if constexpr (!O::kQ8) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
-      uint32_t row = __shfl(rows, key);
-      row = row == ~0u ? 0 : row;
-      const int64_t at = (int64_t)row * c.D * O::kBytes + cc * 16;
-      reg.k[i] = reg.v[i] = u4{0, 0, 0, 0};
-      if (cc < ch) {
-        reg.k[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.k) + at);
-        reg.v[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.v) + at);
+      for (int i = 0; i < NL; ++i) {
+        const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
+        const int64_t at = row_of(rows, key) + cc * 16;
+        kr[i] = vr[i] = u4{0, 0, 0, 0};
+        if (EXACT || cc < ch) {
+          kr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.k) + at);
+          vr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.v) + at);
+        }
       }
     }
-    if constexpr (O::kQ8) {
-      const int nb = c.D / 32;
-      auto scales = [&](const _Float16* p, uint32_t row) {
-        row = row == ~0u ? 0 : row;
-        union { u4 w; _Float16 h[8]; } x;
-        x.w = u4{0, 0, 0, 0};
+  };
+  // (columns past D: any codes, of scale 0)
+  auto load_k = [&](uint32_t rows) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
-          if (i < nb) x.h[i] = p[(int64_t)row * nb + i];
-        return x.w;
-      };
-      reg.ks[0] = scales(c.ks, __shfl(rows, n16));
-      reg.ks[1] = scales(c.ks, __shfl(rows, 16 + n16));
-      reg.vs = scales(c.vs, rows);
+    for (int i = 0; i < NL; ++i) {
+      const int key = (i * 64 + lane) / CH, cc = (k_at<CH>(key, lane % CH) >> 4) % CH;
+      load_to_lds(static_cast<const char*>(c.k) + row_of(rows, key) + (EXACT || cc < ch ? cc : 0) * 16, kt_ + i * 1024);
     }
+    ksc = row_scales<KS, EXACT>(c.ks, rows, c.D / 32);
+  };
+  auto load_v = [&](uint32_t rows) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int key = (i * 64 + lane) / CH, cc = (v_at<CH, true>(key, lane % CH) >> 4) % CH;
+      load_to_lds(static_cast<const char*>(c.v) + row_of(rows, key) + (EXACT || cc < ch ? cc : 0) * 16, vt_ + i * 1024);
+    }
+    vsc = row_scales<KS, EXACT>(c.vs, rows, c.D / 32);
   };
 
-  int kt = k0 + wave * kTile;
+  int kt = k0 + wave * KT;
   uint32_t rows = 0, rows_next = 0;
   if (kt < k1) {
     rows = look_up(kt);
-    load(rows);
-    rows_next = look_up(kt + kStepWaves * kTile);
+    if constexpr (O::kQ8) {
+      load_k(rows);
+      load_v(rows);
+    } else {
+      load(rows);
+    }
+    rows_next = look_up(kt + kStepWaves * KT);
   }
-  for (; kt < k1; kt += kStepWaves * kTile) {
+  for (; kt < k1; kt += kStepWaves * KT) {
     // values of keys outside the rows' span count for none of them, whatever they hold: stored as zeros. So are, in a tile that
     // some rows see in part only, values that are not finite (a weight of 0 times one is NaN), and their keys are noted
-    const bool inside = kt >= lo && kt + kTile <= hi;
-    const bool masked = kt < all_lo || kt + kTile > all_hi || !inside, part = masked && pa != pz;
-    uint32_t odd = 0;
+    const bool inside = kt >= lo && kt + KT <= hi;
+    const bool masked = kt < all_lo || kt + KT > all_hi || !inside, part = masked && pa != pz;
+    const bool more = kt + kStepWaves * KT < k1;
+    uint64_t odd = 0;
+    const uint32_t here = rows;
+    if constexpr (!O::kQ8) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
-      *reinterpret_cast<u4*>(kt_ + k_at<CH>(key, cc)) = reg.k[i];
-      u4 v = reg.v[i];
-      if (!inside && (kt + key < lo || kt + key >= hi)) v = u4{0, 0, 0, 0};
-      if constexpr (!O::kQ8) {
+      for (int i = 0; i < NL; ++i) {
+        const int flat = i * 64 + lane, key = flat / CH, cc = flat % CH;
+        *reinterpret_cast<u4*>(kt_ + k_at<CH>(key, cc)) = kr[i];
+        u4 v = vr[i];
+        if (!inside && (kt + key < lo || kt + key >= hi)) v = u4{0, 0, 0, 0};
         if (part && not_finite<O::kBf16>(v)) {
           v = u4{0, 0, 0, 0};
-          odd |= 1u << key;
+          odd |= 1ull << key;
         }
+        *reinterpret_cast<u4*>(vt_ + v_at<CH, false>(key, cc)) = v;
       }
-      *reinterpret_cast<u4*>(vt_ + v_at<CH, O::kQ8>(key, cc)) = v;
-    }
-    h8 k_scale[2];
-    if constexpr (O::kQ8) {
-      union { u4 w; _Float16 h[8]; } x;
-      x.w = reg.vs;
-      if (lane < 32) {
+      // the next tile's loads, over this tile's registers
+      if (more) {
+        rows = rows_next;
+        load(rows);
+        rows_next = look_up(kt + 2 * kStepWaves * KT);
+      }
+    } else {
+      wait_loads();
+      if (lane < KT) {
         const bool out = kt + lane < lo || kt + lane >= hi;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          _Float16 sc = out ? (_Float16)0.0f : x.h[i];
+          _Float16 sc = out ? (_Float16)0.0f : vsc[i];
           if (part && (__builtin_bit_cast(uint16_t, sc) & 0x7c00u) == 0x7c00u) {
             sc = (_Float16)0.0f;
-            odd |= 1u << lane;
+            odd |= 1ull << lane;
           }
-          vs_[i * kTile + lane] = sc;
+          vs_[i * KT + lane] = sc;
         }
+        ks_[lane] = ksc;
       }
-      k_scale[0] = __builtin_bit_cast(h8, reg.ks[0]);
-      k_scale[1] = __builtin_bit_cast(h8, reg.ks[1]);
-    }
-    const uint32_t here = rows;
-    // the next tile's loads, over this tile's registers
-    if (kt + kStepWaves * kTile < k1) {
-      rows = rows_next;
-      load(rows);
-      rows_next = look_up(kt + 2 * kStepWaves * kTile);
     }
 
-    f4 s[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+    f4 s[NT];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int key = half * 16 + n16;
+    for (int t = 0; t < NT; ++t) {
+      const int key = t * 16 + n16;
+      s[t] = f4{0, 0, 0, 0};
       if constexpr (O::kQ8) {
+        const RowScales<KS> k_scale = ks_[key];
 #pragma unroll
         for (int u = 0; u < KS / 2; ++u) {
           const u4 w = *reinterpret_cast<const u4*>(kt_ + k_at<CH>(key, g + 4 * u));
-          const _Float16 sc = g < 2 ? k_scale[half][2 * u] : k_scale[half][2 * u + 1];
-          const h8 s8_ = {sc, sc, sc, sc, sc, sc, sc, sc};
-          const s8 x = codes_times(u2{w[0], w[1]}, s8_), y = codes_times(u2{w[2], w[3]}, s8_);
-          s[half] = mma16<false>(x, qf[2 * u], s[half]);
-          s[half] = mma16<false>(y, qf[2 * u + 1], s[half]);
+          const _Float16 sc = g < 2 ? k_scale[2 * u] : k_scale[2 * u + 1];  // (of 16 codes of block (g + 4 u) / 2)
+          const h8 sc8 = {sc, sc, sc, sc, sc, sc, sc, sc};
+          s[t] = mma16<false>(codes_times(u2{w[0], w[1]}, sc8), qf[2 * u], s[t]);
+          s[t] = mma16<false>(codes_times(u2{w[2], w[3]}, sc8), qf[2 * u + 1], s[t]);
         }
       } else {
 #pragma unroll
-        for (int u = 0; u < KS; ++u) {
-          const s8 x = *reinterpret_cast<const s8*>(kt_ + k_at<CH>(key, 4 * u + g));
-          s[half] = mma16<O::kBf16>(x, qf[u], s[half]);
-        }
+        for (int u = 0; u < KS; ++u) s[t] = mma16<O::kBf16>(*reinterpret_cast<const s8*>(kt_ + k_at<CH>(key, 4 * u + g)), qf[u], s[t]);
       }
     }
 
-    const bool torn = __ballot(here == ~0u) != 0;  // keys in no page: their scores are NaN
-    uint32_t bad = 0;
-    if (torn) bad = (uint32_t)__ballot(here == ~0u);
+    if constexpr (O::kQ8) {
+      if (more) {  // the next tile's K over this one's, which has been read
+        wait_lds();
+        rows = rows_next;
+        load_k(rows);
+        rows_next = look_up(kt + 2 * kStepWaves * KT);
+      }
+    }
+
+    uint64_t bad = __ballot(here == ~0u);  // keys in no page: their scores are NaN
+    if constexpr (KT < 64) bad &= (1ull << KT) - 1;
     const Scores sc{c_row, cap, slope};
-    float x[8];
+    float x[NT * 4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NT * 4; ++i) {  // key of score i: 16 (i / 4) + 4 g + i % 4
       const int key = (i >> 2) * 16 + g * 4 + (i & 3);
       x[i] = GEN ? sc(s[i >> 2][i & 3], kt + key - pos) : s[i >> 2][i & 3] * c_row;
-      if (torn && (bad >> key & 1)) x[i] = __builtin_nanf("");
-      if (masked && (kt + key < max(see.lo, lo) || kt + key >= min(see.hi, hi))) x[i] = -INFINITY;
+    }
+    if (bad) {
+#pragma unroll
+      for (int i = 0; i < NT * 4; ++i)
+        if (bad >> ((i >> 2) * 16 + g * 4 + (i & 3)) & 1) x[i] = __builtin_nanf("");
+    }
+    if (masked) {
+      const int from = max(see.lo, lo) - kt - g * 4, to = min(see.hi, hi) - kt - g * 4;
+#pragma unroll
+      for (int i = 0; i < NT * 4; ++i) {
+        const int key = (i >> 2) * 16 + (i & 3);
+        if (key < from || key >= to) x[i] = -INFINITY;
+      }
     }
     float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    for (int i = 1; i < NT * 4; ++i) top = fmaxf(top, x[i]);
     top = max_lanes32(max_lanes16(top));
     // the maximum moves only when it is left behind by more than 2^8: weights then stay below 2^8, well inside fp16, and the
     // sums are seldom rescaled
@@ -246,33 +305,45 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= al;
     }
-    float w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = exp2_fast(x[i] - m);
-    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-    const s8 pf = __builtin_bit_cast(s8, u4{pack2<O::kBf16>(w[0], w[1]), pack2<O::kBf16>(w[2], w[3]), pack2<O::kBf16>(w[4], w[5]),
-                                            pack2<O::kBf16>(w[6], w[7])});
+    for (int i = 0; i < NT * 4; ++i) x[i] = exp2_fast(x[i] - m);
+#pragma unroll
+    for (int i = 0; i < NT * 4; i += 4) l += (x[i] + x[i + 1]) + (x[i + 2] + x[i + 3]);
 
-    auto v_frag = [&](int d) -> s8 {
-      if constexpr (O::kQ8) {
-        const int j = n16 >> 1, key = (j & 3) + (j >> 2) * 16 + g * 4;
-        const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((EMBER_LDS(i2)*)(vt_ + v_at<CH, true>(key, d) + (n16 & 1) * 8));
-        const u2 a0 = *reinterpret_cast<const u2*>(vs_ + (d >> 1) * kTile + g * 4);
-        const u2 a1 = *reinterpret_cast<const u2*>(vs_ + (d >> 1) * kTile + 16 + g * 4);
-        return codes_times(u2{(uint32_t)w[0], (uint32_t)w[1]}, __builtin_bit_cast(h8, u4{a0[0], a0[1], a1[0], a1[1]}));
-      } else {
-        const int key = g * 4 + (n16 >> 2), cc = 2 * d + ((n16 >> 1) & 1);
-        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key, cc) + (n16 & 1) * 8));
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key + 16, cc) + (n16 & 1) * 8));
-        return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      }
-    };
+    // by 32 keys: the weights as they lie, and V^T, columns 16 d + n16, its keys in their order
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = mma16<O::kBf16>(v_frag(d), pf, o[d]);
+    for (int q = 0; q < KT / 32; ++q) {
+      const float* const w = x + 8 * q;
+      const s8 pf = __builtin_bit_cast(s8, u4{pack2<O::kBf16>(w[0], w[1]), pack2<O::kBf16>(w[2], w[3]), pack2<O::kBf16>(w[4], w[5]),
+                                              pack2<O::kBf16>(w[6], w[7])});
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        s8 v;
+        if constexpr (O::kQ8) {
+          const int j = n16 >> 1, key = 32 * q + (j & 3) + (j >> 2) * 16 + g * 4;
+          const i2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((EMBER_LDS(i2)*)(vt_ + v_at<CH, true>(key, d) + (n16 & 1) * 8));
+          const _Float16* const at = vs_ + (d >> 1) * KT + 32 * q + g * 4;
+          const u2 a0 = *reinterpret_cast<const u2*>(at), a1 = *reinterpret_cast<const u2*>(at + 16);
+          v = codes_times(u2{(uint32_t)codes[0], (uint32_t)codes[1]}, __builtin_bit_cast(h8, u4{a0[0], a0[1], a1[0], a1[1]}));
+        } else {
+          const int key = 32 * q + g * 4 + (n16 >> 2), cc = 2 * d + ((n16 >> 1) & 1);
+          const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key, cc) + (n16 & 1) * 8));
+          const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vt_ + v_at<CH, false>(key + 16, cc) + (n16 & 1) * 8));
+          v = s8{y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
+        }
+        o[d] = mma16<O::kBf16>(v, pf, o[d]);
+      }
+    }
+    if constexpr (O::kQ8) {
+      if (more) {  // and its V
+        wait_lds();
+        load_v(rows);
+      }
+    }
     if (part && __ballot(odd != 0)) {  // a row that sees one of those keys: NaN by its sum of weights
       for (int k = 32; k; k >>= 1) odd |= __shfl_xor(odd, k);
-      const int from = max(max(see.lo, lo) - kt, 0), to = min(min(see.hi, hi) - kt, kTile);
-      if (from < to && (odd >> from & (~0u >> (32 - (to - from))))) l = __builtin_nanf("");
+      const int from = max(max(see.lo, lo) - kt, 0), to = min(min(see.hi, hi) - kt, KT);
+      if (from < to && (odd >> from & (~0ull >> (64 - (to - from))))) l = __builtin_nanf("");
     }
   }
 
@@ -329,7 +400,7 @@ __global__ __launch_bounds__(kStepThreads, DP <= 128 ? 2 : 1) void attn_step_ker
 template <int T, int IO, int DP>
 int launch_step(const AttnArgs& a, const Parts& p, int part0, int splits, int chunk, int begin, hipStream_t st) {
   const int tiles = (a.c.max_q * a.G + 15) / 16;
-  const dim3 grid(splits * tiles, a.c.n_kv, a.c.n_seqs);
+  const dim3 grid(a.c.n_kv, a.c.n_seqs, splits * tiles);
   const size_t lds = StepLds<T, DP>::kBytes;
   auto go = [&](auto* kernel) {
     if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess)
@@ -337,7 +408,9 @@ int launch_step(const AttnArgs& a, const Parts& p, int part0, int splits, int ch
     kernel<<<grid, kStepThreads, lds, st>>>(a, p, part0, tiles, chunk, begin);
     return hipGetLastError() == hipSuccess ? (int)EMBER_OK : (int)EMBER_ERR_LAUNCH;
   };
-  return a.softcap > 0.0f || a.slopes ? go(attn_step_kernel<T, IO, DP, true>) : go(attn_step_kernel<T, IO, DP, false>);
+  const bool gen = a.softcap > 0.0f || a.slopes;
+  if (a.c.D == DP) return gen ? go(attn_step_kernel<T, IO, DP, true, true>) : go(attn_step_kernel<T, IO, DP, false, true>);
+  return gen ? go(attn_step_kernel<T, IO, DP, true, false>) : go(attn_step_kernel<T, IO, DP, false, false>);
 }
 
 template <int T, int IO>

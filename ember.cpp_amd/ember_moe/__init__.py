@@ -252,6 +252,10 @@ def _stream(stream) -> int:
         return int(stream)
     import torch
 
+    # (torch.cuda.current_stream() builds a stream object, 3 us; this is what it asks)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is not None:
+        return int(raw(torch.cuda.current_device()))
     return int(torch.cuda.current_stream().cuda_stream)
 
 

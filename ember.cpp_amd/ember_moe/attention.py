@@ -61,12 +61,14 @@ def type_id(t) -> int:
     return ty
 
 
-def on_current_device(t) -> None:
+def on_current_device(*tensors) -> None:
     """Refuses tensors that are not on the current device: the library launches there."""
     import torch
 
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise em.EmberError(em.ERR_LAUNCH, f"tensor on {t.device}, the current device is another")
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != here:  # (-1 for a CPU tensor)
+            raise em.EmberError(em.ERR_LAUNCH, f"tensor on {t.device}, the current device is cuda:{here}")
 
 
 def _array(t, n: int, dtype, what: str) -> int:
@@ -92,9 +94,7 @@ def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: int = 
         if pages.dim() != 2 or pages.shape[0] < n:
             raise em.EmberError(em.ERR_SHAPE, "pages: [n_seqs, max_pages] is needed")
         b.pages, b.max_pages = _array(pages, pages.numel(), torch.int32, "pages"), pages.shape[1]
-    for t in (kv_len, q_start, pages):
-        if t is not None:
-            on_current_device(t)
+    on_current_device(*(t for t in (kv_len, q_start, pages) if t is not None))
     b._owner = (kv_len, q_start, pages)
     return b
 
@@ -107,19 +107,18 @@ def attn_options(n_heads: int, head_dim: int, scale: Optional[float] = None, sof
     a = AttnOpts(n_heads=n_heads, scale=head_dim ** -0.5 if scale is None else scale, softcap=softcap, window=window)
     a.slopes = _array(slopes, n_heads, torch.float32, "slopes")
     a.prefix = _array(prefix, 0, torch.int32, "prefix")
-    for t in (slopes, prefix):
-        if t is not None:
-            on_current_device(t)
+    on_current_device(*(t for t in (slopes, prefix) if t is not None))
     a._owner = (slopes, prefix)
     return a
 
 
 def _rows(t, n: int, heads: int, dim: int, what: str) -> int:
     """Checks a [n, heads, dim] tensor whose rows may be apart (a slice of a joint projection); its row stride."""
-    if t.dim() != 3 or t.shape[0] < n or t.shape[1] != heads or t.shape[2] != dim or (heads > 1 and t.stride(1) != dim) or t.stride(2) != 1:
-        raise em.EmberError(em.ERR_SHAPE, f"{what}: [{n}, {heads}, {dim}] with whole rows is needed, got {tuple(t.shape)}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] < n or shape[1] != heads or shape[2] != dim or (heads > 1 and stride[1] != dim) or stride[2] != 1:
+        raise em.EmberError(em.ERR_SHAPE, f"{what}: [{n}, {heads}, {dim}] with whole rows is needed, got {tuple(shape)}")
     # (a single row's stride is anyone's: torch may give 1)
-    return max(t.stride(0), heads * dim) if n <= 1 else t.stride(0)
+    return max(stride[0], heads * dim) if n <= 1 else stride[0]
 
 
 @dataclass
@@ -148,8 +147,7 @@ class DeviceKvCache:
         d = self.desc
         d.type, (d.n_pages, d.n_kv, d.page, d.head_dim) = self.type, shape
         d.k, d.v = self.k.data_ptr(), self.v.data_ptr()
-        for t in (self.k, self.v):
-            on_current_device(t)
+        on_current_device(self.k, self.v)
         if self.type == em.Q8_0:
             for t in (self.k_scale, self.v_scale):
                 if t is None or tuple(t.shape) != shape[:3] + (shape[3] // 32,) or t.dtype != torch.float16 or not t.is_contiguous():
@@ -175,8 +173,7 @@ class DeviceKvCache:
         ks, vs = (_rows(t, batch.n_tokens, d.n_kv, d.head_dim, n) for t, n in ((k, "k"), (v, "v")))
         if k.dtype != v.dtype:
             raise em.EmberError(em.ERR_TYPE, "k and v of one type are needed")
-        for t in (k, v):
-            on_current_device(t)
+        on_current_device(k, v)
         st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, type_id(k), em._stream(stream))
         if st:
             raise em.EmberError(st, fn)
@@ -207,10 +204,9 @@ class DeviceKvCache:
         prefix = getattr(opts, "_owner", (None, None))[1]
         if prefix is not None and prefix.numel() < batch.n_seqs:
             raise em.EmberError(em.ERR_SHAPE, "prefix: one length per sequence is needed")
-        for t in (q, out) if scratch is None else (q, out, scratch):
-            on_current_device(t)
         if scratch is None:
             scratch = torch.empty(max(1, self.attn_scratch_bytes(opts, batch)), dtype=torch.uint8, device=q.device)
+        on_current_device(q, out, scratch)
         st = em.lib().ember_attn(ctypes.byref(opts), ctypes.byref(d), ctypes.byref(batch), q.data_ptr(), qs, out.data_ptr(), os_,
                                  type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream))
         if st:

@@ -57,9 +57,9 @@ typedef struct ember_kv_batch {
   const int32_t* pages;     /* [n_seqs][max_pages] device, or NULL */
   int max_pages;
   /* Attention: the first `shared` tokens of every sequence lie in the same pages, those of sequence 0 (as when
-   * many answers continue one prompt): a multiple of page, 0 if there are none. Their keys and values are then read
-   * once for the whole batch; results are those of the same call with shared = 0. Sequences shorter than `shared`
-   * attend to what they have of it. Needs pages. */
+   * many answers continue one prompt): a multiple of page, 0 if there are none. Where that saves enough,
+   * their keys and values are read once for the whole batch; results are those of the same call with shared = 0, but for
+   * the order of its sums. Sequences shorter than `shared` attend to what they have of it. Needs pages. */
   int shared;
 } ember_kv_batch;
 

@@ -175,6 +175,38 @@ def test_shared(gpu, type_, io, seqs, shared, page, opts):
         case(type_, io, seqs, 8, n_kv, D, page, shared=shared, behind=1, **o)
 
 
+@pytest.mark.parametrize("type_", [em.BF16, em.Q8_0])
+@pytest.mark.parametrize("D,opts", [(128, "plain"), (128, "all"), (64, "plain"), (256, "all")])
+def test_shared_pages_read_once(gpu, type_, D, opts):
+    """Enough sequences behind enough tokens that the shared pages are taken on their own (the scratch says so), some of them
+    shorter than these; q rows of some sequences are several."""
+    n = 220
+    seqs = [(1300, 1)] + [(1280 + (7 * b) % 50, 1 + (b % 9 == 3)) for b in range(1, n)]
+    n_kv, H = (4, 8) if D < 256 else (2, 8)
+    o = {}
+    if opts == "all":
+        o = dict(softcap=20.0, window=700, slopes=torch.tensor([0.5 ** (h + 1) for h in range(H)]), prefix=torch.tensor([30] * n, dtype=torch.int32))
+    s = Setup(type_, seqs, n_kv, D, 64, shared=1216, behind=1).up()
+    short = {5: 1200, 9: 64, 17: 0, 140: 700}
+    lens = [short.get(b, kv) for b, (kv, _) in enumerate(seqs)]
+    s.kv_len.copy_(torch.tensor(lens))
+    dev = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in o.items()}
+    a = em.attn_options(H, D, **dev)
+    with_, alone = s.cache.attn_scratch_bytes(a, s.batch), None
+    s.batch.shared = 0
+    alone = s.cache.attn_scratch_bytes(a, s.batch)
+    s.batch.shared = 1216
+    assert with_ > alone
+    q = rows(s, H, torch.bfloat16)
+    out = torch.full((s.n, H, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = run(s, q.cuda(), H, out, **dev)
+    s.seqs = [(lens[b], nq) for b, (_, nq) in enumerate(seqs)]
+    want, bound = plain_attention(s, q, H, D ** -0.5, heads=[0, H - 1], **o)
+    k = s.starts[-1]
+    check(got[:k, [0, H - 1]], want[:k, [0, H - 1]], bound[:k, [0, H - 1]])
+    assert (got[k:] == 5.0).all()
+
+
 def test_sequences_shorter_than_the_shared_part(gpu):
     s = Setup(em.BF16, [(100, 1), (100, 2), (70, 70)], 2, 64, 16, shared=64)
     s.up()
