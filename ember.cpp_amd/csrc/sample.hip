@@ -3,147 +3,344 @@
 // Everything that decides is exact, so that the result depends on neither the order of the sums nor the grid: logits are
 // compared as order-preserving 32-bit keys, and weights are summed as integers, w_i 2^s rounded once, with s such that
 // a row's V weights (at most 1 each) stay below 2^62. Both filters are thresholds in the descending order: the key at
-// which the count (top-k) or the weight (top-p) of the keys at or above it reaches its share, found digit by digit (11,
-// 11, 10 bits) from a histogram in LDS, and how many of the logits equal to the threshold, by index, still belong.
+// which the count (top-k) or the weight (top-p) of the keys at or above it reaches its share, and how many of the logits equal
+// to it, by index, still belong.
+//
+// A row takes as few passes as its settings allow (one of up to 32768 tokens stays in registers); the first finds the largest logit.
+//   * Where a bound leaves at most kCap tokens (top-k: the k-th largest of the 1024 threads' own maxima is no larger than the k-th
+//     largest logit; min-p alone: its logit; or a short row), a second pass gathers them into LDS, eight a thread, and the
+//     rest works on these.
+//   * Otherwise each filter takes a pass that puts the tokens into 2048 bins of equal width in the logit (by the key's digits, a
+//     wave's lanes would meet in a few bins and wait for each other: 187 us for one row of 32000), and one that gathers the tokens
+//     of the bin that holds the threshold; should that be more than kCap (nearly all logits equal), three passes by the key's
+//     digits. Then the kept tokens are gathered, or if there are too many a pass sums their weights in cells of consecutive tokens.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "ember_sample.h"
 #include "moe_conv.hpp"
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
+constexpr int kPer = 8, kCap = kPer * kThreads;  // gathered tokens
+constexpr int kCell = 256;                       // tokens that a wave takes at once: 4 a lane, side by side
+constexpr int kHeld = 8;                         // cells per wave of a row in registers: 32768 tokens
+constexpr int kLaneMaxK = 900;                   // top-k that the threads' maxima bound well
 typedef unsigned long long u64;
 
 struct Args {
   ember_sampler s;
   const void* z;
-  int type, V;
+  int V;
   int64_t stride;
   const float* u;
   int32_t* ids;
   float* probs;
-  int frac;  // s of the comment above
+  double one;      // 2^s of the comment above, s <= 51
+  int cell_shift;  // the last pass sums cells of kCell << cell_shift tokens, at most kBins of them
 };
 
 // Ascending in the logit; -0 as +0; 0 for what is never drawn (NaN, -inf), so every other key is larger.
-__device__ inline uint32_t key_of(float z) {
+__device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t b = __float_as_uint(z + 0.0f);
   if (z != z || b == 0xff800000u) return 0;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ inline float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
-
-template <int T>
-__device__ inline float logit(const Args& a, int64_t row, int i) {
-  const int64_t at = row * a.stride + i;
-  if constexpr (T == EMBER_TYPE_F32) return static_cast<const float*>(a.z)[at];
-  if constexpr (T == EMBER_TYPE_F16) return (float)static_cast<const _Float16*>(a.z)[at];
-  return ember_moe::bf16_f32(static_cast<const uint16_t*>(a.z)[at]);
-}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 struct Shared {
-  uint32_t cnt[kBins];
-  u64 mass[kBins];
+  u64 bin[kBins];
+  union {
+    struct {
+      uint32_t key[kCap], idx[kCap];
+    };
+    struct {
+      u64 cell[kBins];
+      uint32_t cell_ties[kBins];
+    };
+  };
   u64 wave[kWaves];
-  u64 got[4];
+  u64 got[2];
+  uint32_t count;
 };
 
-template <class F>
-__device__ inline u64 block_sum(Shared& sh, u64 x, F) {
+// The row's keys. ALIGNED: every lane's 4 tokens can be loaded at once. HELD: kept in registers, loaded once.
+template <int T, bool ALIGNED, bool HELD>
+struct Row {
+  const char* p;
+  int V;
+  uint32_t k[HELD ? kHeld : 1][4];
+
+  __device__ __forceinline__ void load(int at, uint32_t (&x)[4]) const {
+    constexpr int size = T == EMBER_TYPE_F32 ? 4 : 2;
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    typedef uint16_t w4 __attribute__((ext_vector_type(4)));
+    const char* const q = p + (int64_t)at * size;
+    float z[4];
+    if (ALIGNED && at + 4 <= V) {
+      if constexpr (T == EMBER_TYPE_F32) {
+        const f4 y = *reinterpret_cast<const f4*>(q);
+        for (int e = 0; e < 4; ++e) z[e] = y[e];
+      } else if constexpr (T == EMBER_TYPE_F16) {
+        const h4 y = *reinterpret_cast<const h4*>(q);
+        for (int e = 0; e < 4; ++e) z[e] = (float)y[e];
+      } else {
+        const w4 y = *reinterpret_cast<const w4*>(q);
+        for (int e = 0; e < 4; ++e) z[e] = ember_moe::bf16_f32(y[e]);
+      }
+    } else {
+      for (int e = 0; e < 4; ++e) {
+        z[e] = -INFINITY;
+        if (at + e >= V) continue;
+        if constexpr (T == EMBER_TYPE_F32) z[e] = reinterpret_cast<const float*>(q)[e];
+        else if constexpr (T == EMBER_TYPE_F16) z[e] = (float)reinterpret_cast<const _Float16*>(q)[e];
+        else z[e] = ember_moe::bf16_f32(reinterpret_cast<const uint16_t*>(q)[e]);
+      }
+    }
+    for (int e = 0; e < 4; ++e) x[e] = key_of(z[e]);
+  }
+  static __device__ int first() { return (int)(threadIdx.x >> 6) * kCell + (int)(threadIdx.x & 63) * 4; }
+  __device__ __forceinline__ void hold() {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int c = 0; c < kHeld; ++c) load(first() + c * kWaves * kCell, k[c]);
+    }
+  }
+  // f(index of the first, keys) for this thread's tokens, 4 at a time; whole waves together.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int c = 0; c < kHeld; ++c)
+        if (c * kWaves * kCell < V) f(first() + c * kWaves * kCell, k[c]);
+    } else {
+      // four cells' loads on the way at once
+      for (int c0 = 0; c0 < V; c0 += 4 * kWaves * kCell) {
+        uint32_t x[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) load(first() + c0 + c * kWaves * kCell, x[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f(first() + c0 + c * kWaves * kCell, x[c]);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ u64 wave_sum(u64 x) {
   for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
-  __syncthreads();
+  return x;
+}
+__device__ __forceinline__ u64 wave_upto(u64 x) {  // over the lanes up to this one
+  const int lane = threadIdx.x & 63;
+  for (int k = 1; k < 64; k <<= 1) {
+    const u64 y = __shfl_up(x, k);
+    if (lane >= k) x += y;
+  }
+  return x;
+}
+// Sum over the block. Ends with a barrier, as the next two.
+__device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
+  x = wave_sum(x);
   if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = x;
   __syncthreads();
   u64 t = 0;
   for (int w = 0; w < kWaves; ++w) t += sh.wave[w];
+  __syncthreads();
   return t;
 }
-// Sum of x over the threads before this one; `total` over all.
-__device__ inline u64 block_before(Shared& sh, u64 x, u64& total) {
+// Of n <= kBins bins, from the highest (down) or lowest on, the one at which the running sum from `run` reaches need: sh.got = {bin, the sum
+// before it}.
+__device__ __forceinline__ void find_bin(Shared& sh, const u64* bins, int n, bool down, u64 run, u64 need) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 inc = x;
-  for (int k = 1; k < 64; k <<= 1) {
-    const u64 y = __shfl_up(inc, k);
-    if (lane >= k) inc += y;
+  u64 x[2] = {0, 0};
+  int b[2];
+  for (int e = 0; e < 2; ++e) {
+    const int at = 2 * (int)threadIdx.x + e;
+    b[e] = down ? n - 1 - at : at;
+    if (at < n) x[e] = bins[b[e]];
+  }
+  const u64 upto = wave_upto(x[0] + x[1]);
+  if (lane == 63) sh.wave[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) run += sh.wave[w];
+  run += upto - x[0] - x[1];
+  for (int e = 0; e < 2; ++e) {
+    if (run < need && run + x[e] >= need) {
+      sh.got[0] = (u64)b[e];
+      sh.got[1] = run;
+    }
+    run += x[e];
   }
   __syncthreads();
-  if (lane == 63) sh.wave[wave] = inc;
+}
+__device__ __forceinline__ void clear_bins(Shared& sh) {
+  sh.bin[threadIdx.x] = 0;
+  sh.bin[kThreads + threadIdx.x] = 0;
   __syncthreads();
-  u64 before = 0;
-  total = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += sh.wave[w];
-    total += sh.wave[w];
-  }
-  return before + inc - x;
 }
 
 struct Weigh {
   float top;
-  double inv_t;
-  int frac;
-  __device__ double e(uint32_t key) const {
+  double inv_t, one;
+  __device__ __forceinline__ double e(uint32_t key) const {
     const float z = value_of(key);
     return z == top ? 1.0 : exp(((double)z - (double)top) * inv_t);
   }
-  __device__ u64 fix(double e) const { return (u64)rint(ldexp(e, frac)); }
+  // e 2^s to the nearest integer: the low bits of 2^52 plus it
+  __device__ __forceinline__ u64 fix(double e) const { return __double_as_longlong(__builtin_fma(e, one, 0x1p52)) - __double_as_longlong(0x1p52); }
 };
 
-// The largest key t whose keys >= t have together at least `need` (by_mass: weight, else count), over the keys above
-// `floor_key`, with `extra` of the floor key itself; `above` gets what the keys > t have.
-template <int T, bool MASS>
-__device__ uint32_t select(const Args& a, int64_t row, Shared& sh, const Weigh& w, uint32_t floor_key, u64 extra, u64 need, u64& above) {
-  const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+// Over the threads' items (amount a[i], 0: none): the largest key t in [lo, hi] whose keys >= t hold `need` together with `above`, which
+// gets what the keys > t hold. Eleven bits of the difference to lo at a time.
+template <int N>
+__device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&key)[N], const u64 (&a)[N], uint32_t lo, uint32_t hi, u64 need, u64& above) {
+  uint32_t width = hi - lo;
+  int s = max(0, 32 - __clz((int)width) - 11);
+  for (;;) {
+    clear_bins(sh);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (a[i] && key[i] - lo <= width) atomicAdd(&sh.bin[(key[i] - lo) >> s], a[i]);  // (a key under lo is far above width)
+    __syncthreads();
+    find_bin(sh, sh.bin, kBins, true, above, need);
+    lo += (uint32_t)sh.got[0] << s;
+    above = sh.got[1];
+    __syncthreads();
+    if (s == 0) return lo;
+    width = (1u << s) - 1;
+    s = max(0, s - 11);
+  }
+}
+
+// Gathers the tokens that `is` picks, in any order; whether they fit.
+template <class R, class F>
+__device__ __forceinline__ bool gather(const R& r, Shared& sh, F is) {
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  r.each([&](int i, const uint32_t (&k)[4]) {
+    uint32_t n = 0;
+    bool in[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      in[e] = k[e] && is(k[e]);
+      n += in[e];
+    }
+    if (!__ballot(n != 0)) return;
+    uint32_t upto = n;
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t y = __shfl_up(upto, s);
+      if ((int)(threadIdx.x & 63) >= s) upto += y;
+    }
+    uint32_t at = 0;
+    if ((threadIdx.x & 63) == 63) at = atomicAdd(&sh.count, upto);
+    at = __shfl(at, 63) + upto - n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (in[e]) {
+        if (at < kCap) {
+          sh.key[at] = k[e];
+          sh.idx[at] = (uint32_t)(i + e);
+        }
+        ++at;
+      }
+  });
+  __syncthreads();
+  const bool fits = sh.count <= kCap;
+  __syncthreads();
+  return fits;
+}
+
+// select_items over the whole row by the key's digits, for the keys above floor_key and `extra` for that key itself. MASS: by weight.
+template <bool MASS, class R>
+__device__ __forceinline__ uint32_t select_row(const R& r, Shared& sh, const Weigh& w, uint32_t floor_key, u64 extra, u64 need, u64& above) {
   uint32_t prefix = 0;
   above = 0;
   for (int p = 0; p < 3; ++p) {
-    const int sh_ = shifts[p], nb = 1 << bits[p];
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.mass[i] = 0;
+    const int s = p == 0 ? 21 : p == 1 ? 10 : 0, bits = p == 2 ? 10 : 11, nb = 1 << bits;
+    clear_bins(sh);
+    r.each([&](int, const uint32_t (&k)[4]) {
+      for (int e = 0; e < 4; ++e)
+        if (k[e] > floor_key && (!p || (k[e] >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(k[e] >> s) & (nb - 1)], MASS ? w.fix(w.e(k[e])) : 1ull);
+    });
+    if (extra && threadIdx.x == 0 && (!p || (floor_key >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(floor_key >> s) & (nb - 1)], extra);
     __syncthreads();
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const uint32_t k = key_of(logit<T>(a, row, i));
-      if (k <= floor_key || k == 0) continue;
-      if (p && (k >> (sh_ + bits[p])) != prefix) continue;
-      atomicAdd(&sh.mass[(k >> sh_) & (nb - 1)], MASS ? w.fix(w.e(k)) : 1ull);
-    }
-    __syncthreads();
-    if (extra && threadIdx.x == 0 && (!p || (floor_key >> (sh_ + bits[p])) == prefix))
-      sh.mass[(floor_key >> sh_) & (nb - 1)] += extra;
-    __syncthreads();
-    // the bin, from the top, at which the running sum reaches `need`: thread t has the bins nb - 1 - 2 t and the one below
-    u64 x[2] = {0, 0};
-    for (int e = 0; e < 2; ++e) {
-      const int bin = nb - 1 - (2 * (int)threadIdx.x + e);
-      if (bin >= 0) x[e] = sh.mass[bin];
-    }
-    u64 total, run = above + block_before(sh, x[0] + x[1], total);
-    for (int e = 0; e < 2; ++e) {
-      const int bin = nb - 1 - (2 * (int)threadIdx.x + e);
-      if (bin >= 0 && run < need && run + x[e] >= need) {
-        sh.got[0] = bin;
-        sh.got[1] = run;
-      }
-      run += x[e];
-    }
-    __syncthreads();
-    prefix = (prefix << bits[p]) | (uint32_t)sh.got[0];
+    find_bin(sh, sh.bin, nb, true, above, need);
+    prefix = (prefix << bits) | (uint32_t)sh.got[0];
     above = sh.got[1];
     __syncthreads();
   }
   return prefix;
 }
 
-template <int T>
+// The same by bins of equal width from the largest logit down to `low`, then the tokens of one of them. MASS: need is set to the share
+// `share` of the whole.
+template <bool MASS, class R>
+__device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const Weigh& w, float low, uint32_t floor_key, u64 extra, double share, u64& need, u64& above) {
+  const float scale = (float)(kBins - 1) / fmaxf(w.top - low, 1e-30f);
+  // (each step of it is monotone in z, rounded or not, and what overflows to NaN comes last, after infinity)
+  auto bin_of = [&](uint32_t k) { return kBins - 1 - (int)fminf((w.top - value_of(k)) * scale, (float)(kBins - 1)); };
+  clear_bins(sh);
+  u64 sum = threadIdx.x == 0 ? extra : 0;
+  r.each([&](int, const uint32_t (&k)[4]) {
+    for (int e = 0; e < 4; ++e)
+      if (k[e] > floor_key) {
+        const u64 x = MASS ? w.fix(w.e(k[e])) : 1ull;
+        if (x) atomicAdd(&sh.bin[bin_of(k[e])], x);
+        sum += x;
+      }
+  });
+  if (extra && threadIdx.x == 0) atomicAdd(&sh.bin[bin_of(floor_key)], extra);
+  if (MASS) need = max(1ull, (u64)ceil(share * (double)block_sum(sh, sum)));
+  else __syncthreads();
+  find_bin(sh, sh.bin, kBins, true, 0, need);
+  const int b = (int)sh.got[0];
+  above = sh.got[1];
+  __syncthreads();
+  if (!gather(r, sh, [&](uint32_t k) { return k > floor_key && bin_of(k) == b; })) return select_row<MASS>(r, sh, w, floor_key, extra, need, above);
+  uint32_t key[kPer], lo = ~0u, hi = 0;
+  u64 x[kPer], here = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t at = i * kThreads + threadIdx.x;
+    key[i] = at < sh.count ? sh.key[at] : 0;
+    x[i] = !key[i] ? 0 : MASS ? w.fix(w.e(key[i])) : 1ull;
+    here += x[i];
+    if (key[i]) lo = min(lo, key[i]), hi = max(hi, key[i]);
+  }
+  if (extra) {  // should the bin's tokens not reach `need`, it is the floor key, in the same bin, that does
+    here = block_sum(sh, here);
+    if (above + here < need) {
+      above += here;
+      return floor_key;
+    }
+  }
+  for (int k = 32; k; k >>= 1) {
+    lo = min(lo, (uint32_t)__shfl_xor((int)lo, k));
+    hi = max(hi, (uint32_t)__shfl_xor((int)hi, k));
+  }
+  if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = (u64)hi << 32 | lo;
+  __syncthreads();
+  for (int v = 0; v < kWaves; ++v) {
+    lo = min(lo, (uint32_t)sh.wave[v]);
+    hi = max(hi, (uint32_t)(sh.wave[v] >> 32));
+  }
+  __syncthreads();
+  return select_items(sh, key, x, lo, hi, need, above);
+}
+
+template <int T, bool ALIGNED, bool HELD>
 __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
-  __shared__ Shared sh;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  Shared& sh = *reinterpret_cast<Shared*>(lds);
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float temp = a.s.temperatures ? a.s.temperatures[row] : a.s.temperature;
-  int top_k = a.s.top_ks ? a.s.top_ks[row] : a.s.top_k;
+  const int top_k = a.s.top_ks ? a.s.top_ks[row] : a.s.top_k;
   float top_p = a.s.top_ps ? a.s.top_ps[row] : a.s.top_p;
   float min_p = a.s.min_ps ? a.s.min_ps[row] : a.s.min_p;
   if (temp != temp) temp = 1.0f;
@@ -152,88 +349,250 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   min_p = fminf(min_p, 1.0f);
   float u = a.u[row];
   u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+  Row<T, ALIGNED, HELD> r;
+  r.p = static_cast<const char*>(a.z) + row * a.stride * (T == EMBER_TYPE_F32 ? 4 : 2);
+  r.V = a.V;
+  r.hold();
 
-  // the largest key, its lowest index, and how many can be drawn at all
-  u64 best = 0;
-  u64 n_valid = 0;
-  for (int i = tid; i < a.V; i += kThreads) {
-    const uint32_t k = key_of(logit<T>(a, row, i));
-    n_valid += k != 0;
-    const u64 x = (u64)k << 32 | (uint32_t)~i;
-    best = x > best ? x : best;
-  }
+  // the largest key, its lowest index, the smallest key that can be drawn, how many can
+  uint32_t best = 0, best_i = 0, least = ~0u, n_valid = 0;
+  r.each([&](int i, const uint32_t (&k)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (k[e] > best) best = k[e], best_i = (uint32_t)(i + e);  // (a thread's indices ascend)
+      if (k[e]) least = min(least, k[e]);
+      n_valid += k[e] != 0;
+    }
+  });
+  const uint32_t my_best = best;
+  u64 first = (u64)best << 32 | (uint32_t)~best_i;
   for (int k = 32; k; k >>= 1) {
-    const u64 o = __shfl_xor(best, k);
-    best = o > best ? o : best;
+    const u64 o = __shfl_xor(first, k);
+    first = o > first ? o : first;
+    least = min(least, (uint32_t)__shfl_xor((int)least, k));
+    n_valid += __shfl_xor((int)n_valid, k);
   }
-  if ((tid & 63) == 0) sh.wave[tid >> 6] = best;
+  if (lane == 0) {
+    sh.wave[wave] = first;
+    sh.bin[wave] = (u64)n_valid << 32 | least;
+  }
   __syncthreads();
-  for (int w = 0; w < kWaves; ++w) best = sh.wave[w] > best ? sh.wave[w] : best;
-  n_valid = block_sum(sh, n_valid, 0);
-  const uint32_t top_key = (uint32_t)(best >> 32);
+  n_valid = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    first = sh.wave[w] > first ? sh.wave[w] : first;
+    least = min(least, (uint32_t)sh.bin[w]);
+    n_valid += (uint32_t)(sh.bin[w] >> 32);
+  }
+  __syncthreads();
+  const uint32_t top_key = (uint32_t)(first >> 32);
   if (top_key == 0 || temp <= 0.0f || top_k == 1 || top_p <= 0.0f) {
     if (tid == 0) {
-      a.ids[row] = top_key ? (int32_t)~(uint32_t)best : -1;
+      a.ids[row] = top_key ? (int32_t)~(uint32_t)first : -1;
       if (a.probs) a.probs[row] = top_key ? 1.0f : 0.0f;
     }
     return;
   }
-  const Weigh w{value_of(top_key), 1.0 / (double)temp, a.frac};
+  const Weigh w{value_of(top_key), 1.0 / (double)temp, a.one};
+  bool by_k = top_k > 0 && (uint32_t)top_k < n_valid, by_p = top_p < 1.0f;
 
-  // the threshold key and how many of the logits equal to it belong
+  // a key that no token to be kept is under: `low` of all, `floor` (0: none) where few tokens are at or above it
+  uint32_t low = least, floor = 0;
+  if (min_p > 0.0f && !by_p && !by_k) {
+    // the logit of weight min_p, less what its rounding may be off by
+    const double z = (double)w.top + (double)temp * log((double)min_p), off = 1e-6 * (fabs(z) + (double)temp);
+    low = floor = max(low, key_of((float)(z - off)));
+  }
+  if (n_valid <= kCap) floor = low;
+  if (by_k && top_k <= kLaneMaxK && !floor) {
+    const uint32_t key[1] = {my_best};
+    const u64 x[1] = {my_best != 0};
+    u64 above = 0;
+    if (block_sum(sh, x[0]) >= (u64)top_k) low = floor = select_items(sh, key, x, least, top_key, (u64)top_k, above);
+  }
+  bool listed = floor && gather(r, sh, [&](uint32_t k) { return k >= floor; });
+  // the threshold key, if it is known before the tokens are gathered, and how many of the logits equal to it belong
   uint32_t t = 0;
-  u64 ties = ~0ull, above;
-  if (top_k > 0 && (u64)top_k < n_valid) {
-    t = select<T, false>(a, row, sh, w, 0, 0, (u64)top_k, above);
-    ties = (u64)top_k - above;
-  }
-  if (top_p < 1.0f) {
-    const u64 wt = t ? w.fix(w.e(t)) : 0, extra = t ? ties * wt : 0;
-    u64 sum = 0;
-    for (int i = tid; i < a.V; i += kThreads) {
-      const uint32_t k = key_of(logit<T>(a, row, i));
-      if (k > t) sum += w.fix(w.e(k));
+  u64 ties = ~0ull;
+  if (!listed && (by_k || by_p)) {
+    u64 need = (u64)top_k, above = 0;
+    if (by_k) {
+      t = threshold_row<false>(r, sh, w, value_of(low), 0, 0, 0.0, need, above);
+      ties = need - above;
     }
-    sum = block_sum(sh, sum, 0) + extra;
-    const u64 need = max(1ull, (u64)ceil((double)top_p * (double)sum));
-    const uint32_t t2 = select<T, true>(a, row, sh, w, t, extra, need, above);
-    const u64 w2 = w.fix(w.e(t2)), n = (need - above + w2 - 1) / w2;
-    ties = t2 == t ? min(ties, n) : n;
-    t = t2;
+    if (by_p) {
+      const u64 extra = t ? ties * w.fix(w.e(t)) : 0;
+      // (weights under e^-43 are 0: tokens further down hold nothing)
+      const uint32_t t2 = threshold_row<true>(r, sh, w, fmaxf(value_of(max(t, low)), w.top - 43.0f * temp), t, extra, (double)top_p, need, above);
+      const u64 each_ = w.fix(w.e(t2)), n = (need - above + each_ - 1) / each_;
+      ties = t2 == t ? min(ties, n) : n;
+      t = t2;
+    }
+    by_k = by_p = false;
+    low = t;
+    listed = gather(r, sh, [&](uint32_t k) { return k >= t; });
   }
 
-  // the kept tokens' weight, tile by tile of 1024 consecutive indices; then the tile, and the token in it
-  auto weight = [&](uint32_t k, u64 rank) -> u64 {  // rank: how many of equal key come before
-    if (k == 0 || k < t || (k == t && rank >= ties)) return 0;
+  if (listed) {
+    uint32_t key[kPer], idx[kPer];  // idx: inverted, so that the first index is the largest
+    u64 x[kPer];
+    const uint32_t n = sh.count, inv_lo = ~(uint32_t)(a.V - 1);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t at = i * kThreads + tid;
+      key[i] = at < n ? sh.key[at] : 0;
+      idx[i] = at < n ? ~sh.idx[at] : 0;
+      x[i] = key[i] != 0;
+    }
+    // keeps of the items equal to t the first `keep` by index, and none under it
+    auto cut = [&](uint32_t t_, u64 keep) {
+      u64 eq[kPer], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (key[i] < t_) x[i] = 0;
+        eq[i] = x[i] && key[i] == t_;
+        mine += eq[i];
+      }
+      if (block_sum(sh, mine) <= keep) return;
+      u64 before = 0;
+      const uint32_t last = select_items(sh, idx, eq, inv_lo, ~0u, keep, before);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (eq[i] && idx[i] < last) x[i] = 0;
+    };
+    if (t) cut(t, ties);
+    if (by_k) {
+      u64 above = 0;
+      const uint32_t t_ = select_items(sh, key, x, low, top_key, (u64)top_k, above);
+      cut(t_, (u64)top_k - above);
+    }
+    uint32_t under = 0;  // bit i: item i has less than min_p
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (x[i]) {
+        const double e = w.e(key[i]);
+        x[i] = w.fix(e);
+        under |= (uint32_t)(e < (double)min_p) << i;
+      }
+    if (by_p) {
+      u64 mine = 0, above = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) mine += x[i];
+      const u64 need = max(1ull, (u64)ceil((double)top_p * (double)block_sum(sh, mine)));
+      const uint32_t t_ = select_items(sh, key, x, low, top_key, need, above);
+      const u64 each_ = w.fix(w.e(t_));
+      cut(t_, (need - above + each_ - 1) / each_);
+    }
+    u64 mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (under >> i & 1) x[i] = 0;
+      mine += x[i];
+    }
+    const u64 sum = block_sum(sh, mine), target = (u64)((double)u * (double)sum);
+    u64 before = 0;
+    const uint32_t drawn = select_items(sh, idx, x, inv_lo, ~0u, target + 1, before);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (x[i] && idx[i] == drawn) {
+        a.ids[row] = (int32_t)~drawn;
+        if (a.probs) a.probs[row] = (float)((double)x[i] / (double)sum);
+      }
+    return;
+  }
+
+  // Too many to gather: the weights of the tokens above t, and the tokens equal to it, by cells of consecutive tokens, a wave a cell.
+  auto weight = [&](uint32_t k) -> u64 {
     const double e = w.e(k);
     return e >= (double)min_p ? w.fix(e) : 0;
   };
-  u64 sum = 0, seen = 0;
-  for (int i0 = 0; i0 < a.V; i0 += kThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < a.V ? key_of(logit<T>(a, row, i)) : 0;
-    u64 n, rank = seen + block_before(sh, t && k == t, n);
-    seen += n;
-    sum += weight(k, rank);
-  }
-  sum = block_sum(sh, sum, 0);
-  const u64 target = (u64)((double)u * (double)sum);
-  u64 run = 0;
-  seen = 0;
-  for (int i0 = 0; i0 < a.V; i0 += kThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < a.V ? key_of(logit<T>(a, row, i)) : 0;
-    u64 n, rank = seen + block_before(sh, t && k == t, n);
-    seen += n;
-    const u64 x = weight(k, rank);
-    const u64 before = run + block_before(sh, x, n);
-    run += n;
-    if (before <= target && target < before + x) {
-      a.ids[row] = i;
-      if (a.probs) a.probs[row] = (float)((double)x / (double)sum);
+  const u64 wt = t ? weight(t) : 0;
+  const int cells = (a.V + (kCell << a.cell_shift) - 1) / (kCell << a.cell_shift);
+  for (int c = wave; c < cells; c += kWaves) {
+    u64 x = 0;
+    uint32_t eq = 0;
+    for (int sub = 0; sub < 1 << a.cell_shift; ++sub) {
+      uint32_t k[4];
+      r.load(((c << a.cell_shift) + sub) * kCell + lane * 4, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (k[e] > t) x += weight(k[e]);
+        eq += t && k[e] == t;
+      }
     }
-    if (run > target) break;
+    x = wave_sum(x);
+    for (int s = 32; s; s >>= 1) eq += __shfl_xor((int)eq, s);
+    if (lane == 0) {
+      sh.cell[c] = x;
+      sh.cell_ties[c] = eq;
+    }
   }
+  __syncthreads();
+  // of the equal ones the first `ties` count: thread c has the cells 2 c and 2 c + 1
+  {
+    u64 n[2] = {0, 0};
+    for (int e = 0; e < 2; ++e)
+      if (2 * tid + e < cells) n[e] = sh.cell_ties[2 * tid + e];
+    const u64 upto = wave_upto(n[0] + n[1]);
+    if (lane == 63) sh.wave[wave] = upto;
+    __syncthreads();
+    u64 before = upto - n[0] - n[1], mine = 0;
+    for (int v = 0; v < wave; ++v) before += sh.wave[v];
+    for (int e = 0; e < 2; ++e) {
+      const int c = 2 * tid + e;
+      const u64 kept = before >= ties ? 0 : min(n[e], ties - before);
+      if (c < cells) {
+        sh.cell[c] += kept * wt;
+        sh.bin[c] = kept;
+        mine += sh.cell[c];
+      }
+      before += n[e];
+    }
+    __syncthreads();
+    const u64 sum = block_sum(sh, mine), target = (u64)((double)u * (double)sum);
+    find_bin(sh, sh.cell, cells, false, 0, target + 1);
+    if (wave) return;
+    const int c = (int)sh.got[0];
+    u64 run = sh.got[1], left = sh.bin[c];
+    for (int sub = 0; sub < 1 << a.cell_shift; ++sub) {
+      uint32_t k[4];
+      const int at = ((c << a.cell_shift) + sub) * kCell + lane * 4;
+      r.load(at, k);
+      uint32_t eq = 0;
+      for (int e = 0; e < 4; ++e) eq += t && k[e] == t;
+      const u64 eq_upto = wave_upto(eq);
+      u64 rank = eq_upto - eq, x[4], mine_ = 0;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = k[e] > t ? weight(k[e]) : 0;
+        if (t && k[e] == t) x[e] = rank++ < left ? wt : 0;
+        mine_ += x[e];
+      }
+      const u64 upto = wave_upto(mine_);
+      u64 at_run = run + upto - mine_;
+      for (int e = 0; e < 4; ++e) {
+        if (at_run <= target && target < at_run + x[e]) {
+          a.ids[row] = at + e;
+          if (a.probs) a.probs[row] = (float)((double)x[e] / (double)sum);
+        }
+        at_run += x[e];
+      }
+      run += __shfl(upto, 63);
+      left -= min(left, (u64)__shfl(eq_upto, 63));
+    }
+  }
+}
+
+template <int T>
+int launch(const Args& a, int n, bool aligned, hipStream_t st) {
+  auto go = [&](auto* kernel) {
+    static_assert(sizeof(Shared) <= 160 * 1024, "LDS of a CU");
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)) != hipSuccess)
+      return (int)EMBER_ERR_LAUNCH;
+    kernel<<<n, kThreads, sizeof(Shared), st>>>(a);
+    return hipGetLastError() == hipSuccess ? (int)EMBER_OK : (int)EMBER_ERR_LAUNCH;
+  };
+  const bool held = a.V <= kHeld * kWaves * kCell;
+  if (aligned) return held ? go(sample_kernel<T, true, true>) : go(sample_kernel<T, true, false>);
+  return held ? go(sample_kernel<T, false, true>) : go(sample_kernel<T, false, false>);
 }
 
 }  // namespace
@@ -250,13 +609,14 @@ extern "C" int ember_sample(const ember_sampler* s, const void* logits, int type
   if (off(logits, size) || off(u, 4) || off(ids, 4) || off(probs, 4) || off(s->temperatures, 4) || off(s->top_ks, 4) ||
       off(s->top_ps, 4) || off(s->min_ps, 4))
     return EMBER_ERR_ALIGN;
-  int bits = 0;
+  int bits = 0, shift = 0;
   while ((1 << bits) < V) ++bits;
-  const Args a{*s, logits, type, V, stride, u, ids, probs, 61 - bits};
+  while (((V + (kCell << shift) - 1) / (kCell << shift)) > kBins) ++shift;
+  const Args a{*s, logits, V, stride, u, ids, probs, (double)(1ull << std::min(51, 61 - bits)), shift};
+  const bool aligned = !off(logits, 4 * size) && (n == 1 || stride % 4 == 0);
   switch (type) {
-    case EMBER_TYPE_F32: sample_kernel<EMBER_TYPE_F32><<<n, kThreads, 0, stream>>>(a); break;
-    case EMBER_TYPE_F16: sample_kernel<EMBER_TYPE_F16><<<n, kThreads, 0, stream>>>(a); break;
-    default: sample_kernel<EMBER_TYPE_BF16><<<n, kThreads, 0, stream>>>(a); break;
+    case EMBER_TYPE_F32: return launch<EMBER_TYPE_F32>(a, n, aligned, stream);
+    case EMBER_TYPE_F16: return launch<EMBER_TYPE_F16>(a, n, aligned, stream);
+    default: return launch<EMBER_TYPE_BF16>(a, n, aligned, stream);
   }
-  return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }

@@ -68,12 +68,10 @@ class Setup:
         """[n, n_kv, D] in 64 bits: positions lo .. hi - 1 of sequence b."""
         hi = self.seqs[b][0] if hi is None else hi
         x, sc = (self.k, self.v)[which], self.scales[which]
-        out = torch.empty(hi - lo, self.n_kv, self.D, dtype=torch.float64)
-        for j in range(lo, hi):
-            p, r = self.place(b, j)
-            row = x[p, :, r].double()
-            out[j - lo] = row * sc[p, :, r].double().repeat_interleave(32, -1) if sc is not None else row
-        return out
+        j = torch.arange(lo, hi)
+        p = self.table[b].long()[j // self.page] if self.paged else torch.full_like(j, b)
+        out = x[p, :, j % self.page].double()
+        return out if sc is None else out * sc[p, :, j % self.page].double().repeat_interleave(32, -1)
 
     def up(self):
         c = lambda t: None if t is None else t.cuda()  # noqa: E731
