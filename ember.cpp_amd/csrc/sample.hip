@@ -7,13 +7,15 @@
 // to it, by index, still belong.
 //
 // A row takes as few passes as its settings allow (one of up to 32768 tokens stays in registers); the first finds the largest logit.
-//   * Where a bound leaves at most kCap tokens (top-k: the k-th largest of the 1024 threads' own maxima is no larger than the k-th
-//     largest logit; min-p alone: its logit; or a short row), a second pass gathers them into LDS, eight a thread, and the
+//   * Where a bound leaves at most kCap tokens (top-k: the k-th largest of 2048 groups' maxima, four a thread, is no larger than the
+//     k-th largest logit; min-p alone: its logit; or a short row), a second pass gathers them into LDS, 16 a thread, and the
 //     rest works on these.
-//   * Otherwise each filter takes a pass that puts the tokens into 2048 bins of equal width in the logit (by the key's digits, a
-//     wave's lanes would meet in a few bins and wait for each other: 187 us for one row of 32000), and one that gathers the tokens
-//     of the bin that holds the threshold; should that be more than kCap (nearly all logits equal), three passes by the key's
-//     digits. Then the kept tokens are gathered, or if there are too many a pass sums their weights in cells of consecutive tokens.
+//   * Otherwise a filter takes a pass that puts the tokens into 2048 bins of equal width in the logit (by the key's digits, a
+//     wave's lanes would meet in a few bins and wait for each other: 187 us for one row of 32000), after which the tokens down to the
+//     bin that holds the threshold are gathered as above; or should they be too many those of that bin alone, for the threshold, or
+//     should even these be (nearly all logits equal), three passes by the key's digits find it.
+//   * Kept tokens that are too many to gather: a pass sums their weights in cells of consecutive tokens.
+// 512 threads: what is between two barriers is short, and eight waves meet sooner than sixteen.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,12 +26,14 @@
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kPer = 8, kCap = kPer * kThreads;  // gathered tokens
+constexpr int kPer = 16, kCap = kPer * kThreads;  // gathered tokens
 constexpr int kCell = 256;                       // tokens that a wave takes at once: 4 a lane, side by side
-constexpr int kHeld = 8;                         // cells per wave of a row in registers: 32768 tokens
-constexpr int kLaneMaxK = 900;                   // top-k that the threads' maxima bound well
+constexpr int kHeld = 16;                        // cells per wave of a row in registers: 32768 tokens
+constexpr int kAhead = 16;                       // cells per wave whose loads are on the way at once: 128 KB per block
+constexpr int kBinPer = kBins / kThreads;
+constexpr int kGroupMaxK = 1600;                 // top-k that the maxima of 2048 groups bound well
 typedef unsigned long long u64;
 
 struct Args {
@@ -63,25 +67,25 @@ struct Shared {
       uint32_t cell_ties[kBins];
     };
   };
-  u64 wave[kWaves];
-  u64 got[2];
+  u64 wave[kWaves], meta[kWaves];
+  u64 got[3];
   uint32_t count;
 };
 
-// The row's keys. ALIGNED: every lane's 4 tokens can be loaded at once. HELD: kept in registers, loaded once.
+// The row's logits, -inf past its end. ALIGNED: every lane's 4 tokens can be loaded at once. HELD: kept in registers, loaded once. (Passes compare
+// logits, not keys: 2 instructions a token where the keys took 13, and a pass over 131072 tokens 11 us of nothing else. NaN compares false.)
 template <int T, bool ALIGNED, bool HELD>
 struct Row {
   const char* p;
   int V;
-  uint32_t k[HELD ? kHeld : 1][4];
+  float z[HELD ? kHeld : 1][4];
 
-  __device__ __forceinline__ void load(int at, uint32_t (&x)[4]) const {
+  __device__ __forceinline__ void load(int at, float (&z)[4]) const {
     constexpr int size = T == EMBER_TYPE_F32 ? 4 : 2;
     typedef float f4 __attribute__((ext_vector_type(4)));
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     typedef uint16_t w4 __attribute__((ext_vector_type(4)));
     const char* const q = p + (int64_t)at * size;
-    float z[4];
     if (ALIGNED && at + 4 <= V) {
       if constexpr (T == EMBER_TYPE_F32) {
         const f4 y = *reinterpret_cast<const f4*>(q);
@@ -102,93 +106,118 @@ struct Row {
         else z[e] = ember_moe::bf16_f32(reinterpret_cast<const uint16_t*>(q)[e]);
       }
     }
-    for (int e = 0; e < 4; ++e) x[e] = key_of(z[e]);
   }
   static __device__ int first() { return (int)(threadIdx.x >> 6) * kCell + (int)(threadIdx.x & 63) * 4; }
   __device__ __forceinline__ void hold() {
     if constexpr (HELD) {
 #pragma unroll
-      for (int c = 0; c < kHeld; ++c) load(first() + c * kWaves * kCell, k[c]);
+      for (int c = 0; c < kHeld; ++c) load(first() + c * kWaves * kCell, z[c]);
     }
   }
-  // f(index of the first, keys) for this thread's tokens, 4 at a time; whole waves together.
+  // f(index of the first, logits) for this thread's tokens, 4 at a time; whole waves together.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     if constexpr (HELD) {
 #pragma unroll
       for (int c = 0; c < kHeld; ++c)
-        if (c * kWaves * kCell < V) f(first() + c * kWaves * kCell, k[c]);
+        if (c * kWaves * kCell < V) f(first() + c * kWaves * kCell, z[c]);
     } else {
-      // four cells' loads on the way at once
-      for (int c0 = 0; c0 < V; c0 += 4 * kWaves * kCell) {
-        uint32_t x[4][4];
+      for (int c0 = 0; c0 < V; c0 += kAhead * kWaves * kCell) {
+        float x[kAhead][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) load(first() + c0 + c * kWaves * kCell, x[c]);
+        for (int c = 0; c < kAhead; ++c) load(first() + c0 + c * kWaves * kCell, x[c]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) f(first() + c0 + c * kWaves * kCell, x[c]);
+        for (int c = 0; c < kAhead; ++c)
+          if (c0 + c * kWaves * kCell < V) f(first() + c0 + c * kWaves * kCell, x[c]);
       }
     }
   }
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-  for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k);
-  return x;
+// x of lane l - N of the row of 16 (N < 16), or of the last lane of the row before (rows 1 and 3; or 2 and 3, from lane 31); 0 for none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ u64 wave_upto(u64 x) {  // over the lanes up to this one
-  const int lane = threadIdx.x & 63;
-  for (int k = 1; k < 64; k <<= 1) {
-    const u64 y = __shfl_up(x, k);
-    if (lane >= k) x += y;
-  }
-  return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 from_lane(u64 x) {
+  return (u64)from_lane<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | from_lane<CTRL, ROWS>((uint32_t)x);
 }
-// Sum over the block. Ends with a barrier, as the next two.
+// f over the lanes up to this one (0 leaves a value as it is). By data-parallel moves: the shuffles go through LDS, 6 of them one after
+// the other some 900 cycles for 64 bits.
+template <class V, class F>
+__device__ __forceinline__ V wave_scan(V x, F f) {
+  x = f(x, from_lane<0x111, 0xf>(x));
+  x = f(x, from_lane<0x112, 0xf>(x));
+  x = f(x, from_lane<0x114, 0xf>(x));
+  x = f(x, from_lane<0x118, 0xf>(x));
+  x = f(x, from_lane<0x142, 0xa>(x));
+  return f(x, from_lane<0x143, 0xc>(x));
+}
+__device__ __forceinline__ u64 last_lane(u64 x) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+template <class V>
+__device__ __forceinline__ V wave_upto(V x) {
+  return wave_scan(x, [](V p, V q) { return p + q; });
+}
+template <class V>
+__device__ __forceinline__ V wave_sum(V x) {
+  return last_lane(wave_upto(x));
+}
+template <class V>
+__device__ __forceinline__ V wave_max(V x) {
+  return last_lane(wave_scan(x, [](V p, V q) { return p > q ? p : q; }));
+}
+// Sum over the block. Ends with a barrier, as find_bin.
 __device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
   x = wave_sum(x);
   if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = x;
   __syncthreads();
   u64 t = 0;
+#pragma unroll
   for (int w = 0; w < kWaves; ++w) t += sh.wave[w];
   __syncthreads();
   return t;
 }
 // Of n <= kBins bins, from the highest (down) or lowest on, the one at which the running sum from `run` reaches need: sh.got = {bin, the sum
-// before it}.
-__device__ __forceinline__ void find_bin(Shared& sh, const u64* bins, int n, bool down, u64 run, u64 need) {
+// before it, the sum with it}. Leaves the bins cleared.
+__device__ __forceinline__ void find_bin(Shared& sh, u64* bins, int n, bool down, u64 run, u64 need) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 x[2] = {0, 0};
-  int b[2];
-  for (int e = 0; e < 2; ++e) {
-    const int at = 2 * (int)threadIdx.x + e;
+  u64 x[kBinPer], mine = 0;
+  int b[kBinPer];
+#pragma unroll
+  for (int e = 0; e < kBinPer; ++e) {
+    const int at = kBinPer * (int)threadIdx.x + e;
     b[e] = down ? n - 1 - at : at;
-    if (at < n) x[e] = bins[b[e]];
+    x[e] = at < n ? bins[b[e]] : 0;
+    if (at < n) bins[b[e]] = 0;
+    mine += x[e];
   }
-  const u64 upto = wave_upto(x[0] + x[1]);
+  const u64 upto = wave_upto(mine);
   if (lane == 63) sh.wave[wave] = upto;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) run += sh.wave[w];
-  run += upto - x[0] - x[1];
-  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) run += w < wave ? sh.wave[w] : 0;
+  run += upto - mine;
+#pragma unroll
+  for (int e = 0; e < kBinPer; ++e) {
     if (run < need && run + x[e] >= need) {
       sh.got[0] = (u64)b[e];
       sh.got[1] = run;
+      sh.got[2] = run + x[e];
     }
     run += x[e];
   }
-  __syncthreads();
-}
-__device__ __forceinline__ void clear_bins(Shared& sh) {
-  sh.bin[threadIdx.x] = 0;
-  sh.bin[kThreads + threadIdx.x] = 0;
   __syncthreads();
 }
 
 struct Weigh {
   float top;
   double inv_t, one;
-  __device__ __forceinline__ double e(uint32_t key) const {
-    const float z = value_of(key);
+  __device__ __forceinline__ double e(uint32_t key) const { return at(value_of(key)); }
+  __device__ __forceinline__ double at(float z) const {
     return z == top ? 1.0 : exp(((double)z - (double)top) * inv_t);
   }
   // e 2^s to the nearest integer: the low bits of 2^52 plus it
@@ -202,7 +231,6 @@ __device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&ke
   uint32_t width = hi - lo;
   int s = max(0, 32 - __clz((int)width) - 11);
   for (;;) {
-    clear_bins(sh);
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (a[i] && key[i] - lo <= width) atomicAdd(&sh.bin[(key[i] - lo) >> s], a[i]);  // (a key under lo is far above width)
@@ -210,40 +238,34 @@ __device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&ke
     find_bin(sh, sh.bin, kBins, true, above, need);
     lo += (uint32_t)sh.got[0] << s;
     above = sh.got[1];
-    __syncthreads();
     if (s == 0) return lo;
     width = (1u << s) - 1;
     s = max(0, s - 11);
   }
 }
 
-// Gathers the tokens that `is` picks, in any order; whether they fit.
+// Gathers the tokens that `is` picks (by their logit; none that is never drawn), in any order; whether they fit.
 template <class R, class F>
 __device__ __forceinline__ bool gather(const R& r, Shared& sh, F is) {
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
-  r.each([&](int i, const uint32_t (&k)[4]) {
+  r.each([&](int i, const float (&z)[4]) {
     uint32_t n = 0;
     bool in[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      in[e] = k[e] && is(k[e]);
-      n += in[e];
-    }
-    if (!__ballot(n != 0)) return;
-    uint32_t upto = n;
-    for (int s = 1; s < 64; s <<= 1) {
-      const uint32_t y = __shfl_up(upto, s);
-      if ((int)(threadIdx.x & 63) >= s) upto += y;
-    }
+    for (int e = 0; e < 4; ++e) in[e] = is(z[e]);
+    if (!__ballot(in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n += in[e];
+    const uint32_t upto = wave_upto(n);
     uint32_t at = 0;
     if ((threadIdx.x & 63) == 63) at = atomicAdd(&sh.count, upto);
-    at = __shfl(at, 63) + upto - n;
+    at = last_lane(at) + upto - n;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (in[e]) {
         if (at < kCap) {
-          sh.key[at] = k[e];
+          sh.key[at] = key_of(z[e]);
           sh.idx[at] = (uint32_t)(i + e);
         }
         ++at;
@@ -262,46 +284,62 @@ __device__ __forceinline__ uint32_t select_row(const R& r, Shared& sh, const Wei
   above = 0;
   for (int p = 0; p < 3; ++p) {
     const int s = p == 0 ? 21 : p == 1 ? 10 : 0, bits = p == 2 ? 10 : 11, nb = 1 << bits;
-    clear_bins(sh);
-    r.each([&](int, const uint32_t (&k)[4]) {
-      for (int e = 0; e < 4; ++e)
-        if (k[e] > floor_key && (!p || (k[e] >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(k[e] >> s) & (nb - 1)], MASS ? w.fix(w.e(k[e])) : 1ull);
+    r.each([&](int, const float (&z)[4]) {
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t k = key_of(z[e]);
+        if (k > floor_key && (!p || (k >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(k >> s) & (nb - 1)], MASS ? w.fix(w.at(z[e])) : 1ull);
+      }
     });
     if (extra && threadIdx.x == 0 && (!p || (floor_key >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(floor_key >> s) & (nb - 1)], extra);
     __syncthreads();
     find_bin(sh, sh.bin, nb, true, above, need);
     prefix = (prefix << bits) | (uint32_t)sh.got[0];
     above = sh.got[1];
-    __syncthreads();
   }
   return prefix;
 }
 
-// The same by bins of equal width from the largest logit down to `low`, then the tokens of one of them. MASS: need is set to the share
-// `share` of the whole.
-template <bool MASS, class R>
-__device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const Weigh& w, float low, uint32_t floor_key, u64 extra, double share, u64& need, u64& above) {
-  const float scale = (float)(kBins - 1) / fmaxf(w.top - low, 1e-30f);
+// Bins of equal width from the largest logit down to `low`.
+struct Bins {
+  float top, scale;
+  __device__ __forceinline__ Bins(float top_, float low) : top(top_), scale((float)(kBins - 1) / fmaxf(top_ - low, 1e-30f)) {}
   // (each step of it is monotone in z, rounded or not, and what overflows to NaN comes last, after infinity)
-  auto bin_of = [&](uint32_t k) { return kBins - 1 - (int)fminf((w.top - value_of(k)) * scale, (float)(kBins - 1)); };
-  clear_bins(sh);
+  __device__ __forceinline__ int operator()(float z) const { return kBins - 1 - (int)fminf((top - z) * scale, (float)(kBins - 1)); }
+  // a logit that none of the tokens in bin b and higher ones is under
+  __device__ __forceinline__ float from(int b) const {
+    if (b == 0) return -3.4028235e38f;
+    const float z = top - (float)(kBins - b) / scale;
+    return fmaxf(z - 1e-5f * (fabsf(z) + fabsf(top)), -3.4028235e38f);  // (the steps' roundings: some 2^-22 of either)
+  }
+};
+
+// The bin that holds the threshold, of the keys above floor_key and `extra` for that key itself: sh.got as by find_bin. MASS: by weight, need
+// being set to the share `share` of the whole.
+template <bool MASS, class R>
+__device__ __forceinline__ void bins_row(const R& r, Shared& sh, const Weigh& w, const Bins& bin_of, uint32_t floor_key, u64 extra, double share, u64& need) {
   u64 sum = threadIdx.x == 0 ? extra : 0;
-  r.each([&](int, const uint32_t (&k)[4]) {
+  const float above = floor_key ? value_of(floor_key) : -INFINITY;
+  r.each([&](int, const float (&z)[4]) {
+#pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (k[e] > floor_key) {
-        const u64 x = MASS ? w.fix(w.e(k[e])) : 1ull;
-        if (x) atomicAdd(&sh.bin[bin_of(k[e])], x);
+      if (z[e] > above) {
+        const u64 x = MASS ? w.fix(w.at(z[e])) : 1ull;
+        if (x) atomicAdd(&sh.bin[bin_of(z[e])], x);
         sum += x;
       }
   });
-  if (extra && threadIdx.x == 0) atomicAdd(&sh.bin[bin_of(floor_key)], extra);
+  if (extra && threadIdx.x == 0) atomicAdd(&sh.bin[bin_of(above)], extra);
   if (MASS) need = max(1ull, (u64)ceil(share * (double)block_sum(sh, sum)));
   else __syncthreads();
   find_bin(sh, sh.bin, kBins, true, 0, need);
-  const int b = (int)sh.got[0];
-  above = sh.got[1];
-  __syncthreads();
-  if (!gather(r, sh, [&](uint32_t k) { return k > floor_key && bin_of(k) == b; })) return select_row<MASS>(r, sh, w, floor_key, extra, need, above);
+}
+
+// The threshold itself, in bin b with `above` before it.
+template <bool MASS, class R>
+__device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const Weigh& w, const Bins& bin_of, int b, uint32_t floor_key, u64 extra, u64 need,
+                                                  u64& above) {
+  const float under = floor_key ? value_of(floor_key) : -INFINITY;
+  if (!gather(r, sh, [&](float z) { return z > under && bin_of(z) == b; })) return select_row<MASS>(r, sh, w, floor_key, extra, need, above);
   uint32_t key[kPer], lo = ~0u, hi = 0;
   u64 x[kPer], here = 0;
 #pragma unroll
@@ -319,12 +357,11 @@ __device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const 
       return floor_key;
     }
   }
-  for (int k = 32; k; k >>= 1) {
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, k));
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, k));
-  }
+  lo = ~wave_max(~lo);
+  hi = wave_max(hi);
   if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = (u64)hi << 32 | lo;
   __syncthreads();
+#pragma unroll
   for (int v = 0; v < kWaves; ++v) {
     lo = min(lo, (uint32_t)sh.wave[v]);
     hi = max(hi, (uint32_t)(sh.wave[v] >> 32));
@@ -354,40 +391,49 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   r.V = a.V;
   r.hold();
 
-  // the largest key, its lowest index, the smallest key that can be drawn, how many can
-  uint32_t best = 0, best_i = 0, least = ~0u, n_valid = 0;
-  r.each([&](int i, const uint32_t (&k)[4]) {
+  // the largest logit of the row and of this thread's four groups, which four tokens first held its largest, how many can be drawn
+#pragma unroll
+  for (int i = 0; i < kBinPer; ++i) sh.bin[i * kThreads + tid] = 0;
+  float group[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, best = -INFINITY;
+  uint32_t best_i = 0, n_valid = 0;
+  r.each([&](int i, const float (&z)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (k[e] > best) best = k[e], best_i = (uint32_t)(i + e);  // (a thread's indices ascend)
-      if (k[e]) least = min(least, k[e]);
-      n_valid += k[e] != 0;
+      group[e] = fmaxf(group[e], z[e]);
+      n_valid += (uint32_t)__popcll(__ballot(z[e] > -INFINITY));  // (the wave's)
     }
+    const float m = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+    if (m > best) best = m, best_i = (uint32_t)i;  // (a thread's indices ascend)
   });
-  const uint32_t my_best = best;
-  u64 first = (u64)best << 32 | (uint32_t)~best_i;
-  for (int k = 32; k; k >>= 1) {
-    const u64 o = __shfl_xor(first, k);
-    first = o > first ? o : first;
-    least = min(least, (uint32_t)__shfl_xor((int)least, k));
-    n_valid += __shfl_xor((int)n_valid, k);
-  }
+  uint32_t group_key[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) group_key[e] = key_of(group[e]);
+  u64 first = wave_max((u64)key_of(best) << 32 | (uint32_t)~best_i);
+  // the smallest of the groups' largest (0: a group without a token that can be drawn)
+  uint32_t least = ~wave_max(~min(min(group_key[0], group_key[1]), min(group_key[2], group_key[3])));
   if (lane == 0) {
     sh.wave[wave] = first;
-    sh.bin[wave] = (u64)n_valid << 32 | least;
+    sh.meta[wave] = (u64)n_valid << 32 | least;
   }
   __syncthreads();
   n_valid = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    first = sh.wave[w] > first ? sh.wave[w] : first;
-    least = min(least, (uint32_t)sh.bin[w]);
-    n_valid += (uint32_t)(sh.bin[w] >> 32);
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    first = sh.wave[v] > first ? sh.wave[v] : first;
+    least = min(least, (uint32_t)sh.meta[v]);
+    n_valid += (uint32_t)(sh.meta[v] >> 32);
   }
   __syncthreads();
   const uint32_t top_key = (uint32_t)(first >> 32);
   if (top_key == 0 || temp <= 0.0f || top_k == 1 || top_p <= 0.0f) {
     if (tid == 0) {
-      a.ids[row] = top_key ? (int32_t)~(uint32_t)first : -1;
+      int id = -1;
+      if (top_key) {  // the first of the four
+        float z[4];
+        r.load((int)~(uint32_t)first, z);
+        id = (int)~(uint32_t)first + (key_of(z[0]) == top_key ? 0 : key_of(z[1]) == top_key ? 1 : key_of(z[2]) == top_key ? 2 : 3);
+      }
+      a.ids[row] = id;
       if (a.probs) a.probs[row] = top_key ? 1.0f : 0.0f;
     }
     return;
@@ -396,40 +442,64 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   bool by_k = top_k > 0 && (uint32_t)top_k < n_valid, by_p = top_p < 1.0f;
 
   // a key that no token to be kept is under: `low` of all, `floor` (0: none) where few tokens are at or above it
-  uint32_t low = least, floor = 0;
+  uint32_t low = 1, floor = 0;
   if (min_p > 0.0f && !by_p && !by_k) {
     // the logit of weight min_p, less what its rounding may be off by
     const double z = (double)w.top + (double)temp * log((double)min_p), off = 1e-6 * (fabs(z) + (double)temp);
     low = floor = max(low, key_of((float)(z - off)));
   }
   if (n_valid <= kCap) floor = low;
-  if (by_k && top_k <= kLaneMaxK && !floor) {
-    const uint32_t key[1] = {my_best};
-    const u64 x[1] = {my_best != 0};
+  if (by_k && top_k <= kGroupMaxK && !floor) {
+    u64 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = group_key[e] != 0;
     u64 above = 0;
-    if (block_sum(sh, x[0]) >= (u64)top_k) low = floor = select_items(sh, key, x, least, top_key, (u64)top_k, above);
+    if (block_sum(sh, x[0] + x[1] + x[2] + x[3]) >= (u64)top_k) low = floor = select_items(sh, group_key, x, max(least, 1u), top_key, (u64)top_k, above);
   }
-  bool listed = floor && gather(r, sh, [&](uint32_t k) { return k >= floor; });
-  // the threshold key, if it is known before the tokens are gathered, and how many of the logits equal to it belong
+  auto from = [](float bound) { return [bound](float z) { return z >= bound; }; };
+  // (key 1 is a NaN's neighbour: the lowest logit that can be drawn)
+  bool listed = floor && gather(r, sh, from(floor == 1 ? -3.4028235e38f : value_of(floor)));
+  // of the threshold key, if it is known before the tokens are gathered, how many of the logits equal to it belong; the weight that top-p
+  // needs, if it is known (0: not)
   uint32_t t = 0;
-  u64 ties = ~0ull;
-  if (!listed && (by_k || by_p)) {
-    u64 need = (u64)top_k, above = 0;
-    if (by_k) {
-      t = threshold_row<false>(r, sh, w, value_of(low), 0, 0, 0.0, need, above);
+  u64 ties = ~0ull, need_p = 0;
+  if (!listed && by_k) {
+    u64 need = (u64)top_k;
+    // (twice as far down as the groups' largest reach: what is further comes into the last bin)
+    const float reach = least > 1 ? w.top - 2.0f * (w.top - value_of(least)) : -3.4028235e38f;
+    const Bins bin_of(w.top, fmaxf(reach, low > 1 ? value_of(low) : reach));
+    bins_row<false>(r, sh, w, bin_of, 0, 0, 0.0, need);
+    const int b = (int)sh.got[0];
+    u64 above = sh.got[1];
+    const u64 upto = sh.got[2];
+    if (upto <= kCap) {
+      listed = gather(r, sh, from(bin_of.from(b)));
+    }
+    if (!listed) {
+      t = threshold_row<false>(r, sh, w, bin_of, b, 0, 0, need, above);
       ties = need - above;
+      by_k = false;
+      low = t;
+      // (the k tokens and the ties)
+      if ((u64)top_k <= kCap) listed = gather(r, sh, from(value_of(t)));
     }
-    if (by_p) {
-      const u64 extra = t ? ties * w.fix(w.e(t)) : 0;
-      // (weights under e^-43 are 0: tokens further down hold nothing)
-      const uint32_t t2 = threshold_row<true>(r, sh, w, fmaxf(value_of(max(t, low)), w.top - 43.0f * temp), t, extra, (double)top_p, need, above);
-      const u64 each_ = w.fix(w.e(t2)), n = (need - above + each_ - 1) / each_;
+  }
+  if (!listed && by_p) {
+    // (weights under e^-43 are 0: tokens further down hold nothing)
+    const u64 extra = t ? ties * w.fix(w.e(t)) : 0;
+    const Bins bin_of(w.top, fmaxf(max(t, low) > 1 ? value_of(max(t, low)) : -3.4028235e38f, w.top - 43.0f * temp));
+    bins_row<true>(r, sh, w, bin_of, t, extra, (double)top_p, need_p);
+    const int b = (int)sh.got[0];
+    u64 above = sh.got[1];
+    if (!t) listed = gather(r, sh, from(bin_of.from(b)));
+    if (!listed) {
+      const uint32_t t2 = threshold_row<true>(r, sh, w, bin_of, b, t, extra, need_p, above);
+      const u64 each_ = w.fix(w.e(t2)), n = (need_p - above + each_ - 1) / each_;
       ties = t2 == t ? min(ties, n) : n;
-      t = t2;
+      t = low = t2;
+      by_p = false;
+      listed = gather(r, sh, from(value_of(t)));
     }
-    by_k = by_p = false;
-    low = t;
-    listed = gather(r, sh, [&](uint32_t k) { return k >= t; });
   }
 
   if (listed) {
@@ -477,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
       u64 mine = 0, above = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) mine += x[i];
-      const u64 need = max(1ull, (u64)ceil((double)top_p * (double)block_sum(sh, mine)));
+      const u64 need = need_p ? need_p : max(1ull, (u64)ceil((double)top_p * (double)block_sum(sh, mine)));
       const uint32_t t_ = select_items(sh, key, x, low, top_key, need, above);
       const u64 each_ = w.fix(w.e(t_));
       cut(t_, (need - above + each_ - 1) / each_);
@@ -501,44 +571,49 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   }
 
   // Too many to gather: the weights of the tokens above t, and the tokens equal to it, by cells of consecutive tokens, a wave a cell.
-  auto weight = [&](uint32_t k) -> u64 {
-    const double e = w.e(k);
+  auto weight = [&](float z) -> u64 {
+    const double e = w.at(z);
     return e >= (double)min_p ? w.fix(e) : 0;
   };
-  const u64 wt = t ? weight(t) : 0;
+  const float tz = t ? value_of(t) : -INFINITY;
+  const u64 wt = t ? weight(tz) : 0;
   const int cells = (a.V + (kCell << a.cell_shift) - 1) / (kCell << a.cell_shift);
   for (int c = wave; c < cells; c += kWaves) {
     u64 x = 0;
     uint32_t eq = 0;
     for (int sub = 0; sub < 1 << a.cell_shift; ++sub) {
-      uint32_t k[4];
-      r.load(((c << a.cell_shift) + sub) * kCell + lane * 4, k);
+      float z[4];
+      r.load(((c << a.cell_shift) + sub) * kCell + lane * 4, z);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (k[e] > t) x += weight(k[e]);
-        eq += t && k[e] == t;
+        if (z[e] > tz) x += weight(z[e]);
+        eq += t && z[e] == tz;
       }
     }
     x = wave_sum(x);
-    for (int s = 32; s; s >>= 1) eq += __shfl_xor((int)eq, s);
+    eq = wave_sum(eq);
     if (lane == 0) {
       sh.cell[c] = x;
       sh.cell_ties[c] = eq;
     }
   }
   __syncthreads();
-  // of the equal ones the first `ties` count: thread c has the cells 2 c and 2 c + 1
+  // of the equal ones the first `ties` count
   {
-    u64 n[2] = {0, 0};
-    for (int e = 0; e < 2; ++e)
-      if (2 * tid + e < cells) n[e] = sh.cell_ties[2 * tid + e];
-    const u64 upto = wave_upto(n[0] + n[1]);
+    u64 n[kBinPer], all = 0;
+#pragma unroll
+    for (int e = 0; e < kBinPer; ++e) {
+      n[e] = kBinPer * tid + e < cells ? sh.cell_ties[kBinPer * tid + e] : 0;
+      all += n[e];
+    }
+    const u64 upto = wave_upto(all);
     if (lane == 63) sh.wave[wave] = upto;
     __syncthreads();
-    u64 before = upto - n[0] - n[1], mine = 0;
+    u64 before = upto - all, mine = 0;
     for (int v = 0; v < wave; ++v) before += sh.wave[v];
-    for (int e = 0; e < 2; ++e) {
-      const int c = 2 * tid + e;
+#pragma unroll
+    for (int e = 0; e < kBinPer; ++e) {
+      const int c = kBinPer * tid + e;
       const u64 kept = before >= ties ? 0 : min(n[e], ties - before);
       if (c < cells) {
         sh.cell[c] += kept * wt;
@@ -554,16 +629,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     const int c = (int)sh.got[0];
     u64 run = sh.got[1], left = sh.bin[c];
     for (int sub = 0; sub < 1 << a.cell_shift; ++sub) {
-      uint32_t k[4];
+      float z[4];
       const int at = ((c << a.cell_shift) + sub) * kCell + lane * 4;
-      r.load(at, k);
+      r.load(at, z);
       uint32_t eq = 0;
-      for (int e = 0; e < 4; ++e) eq += t && k[e] == t;
-      const u64 eq_upto = wave_upto(eq);
+      for (int e = 0; e < 4; ++e) eq += t && z[e] == tz;
+      const uint32_t eq_upto = wave_upto(eq);
       u64 rank = eq_upto - eq, x[4], mine_ = 0;
       for (int e = 0; e < 4; ++e) {
-        x[e] = k[e] > t ? weight(k[e]) : 0;
-        if (t && k[e] == t) x[e] = rank++ < left ? wt : 0;
+        x[e] = z[e] > tz ? weight(z[e]) : 0;
+        if (t && z[e] == tz) x[e] = rank++ < left ? wt : 0;
         mine_ += x[e];
       }
       const u64 upto = wave_upto(mine_);
@@ -575,8 +650,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
         }
         at_run += x[e];
       }
-      run += __shfl(upto, 63);
-      left -= min(left, (u64)__shfl(eq_upto, 63));
+      run += last_lane(upto);
+      left -= min(left, (u64)last_lane(eq_upto));
     }
   }
 }
