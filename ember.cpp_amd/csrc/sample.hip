@@ -6,7 +6,7 @@
 // which the count (top-k) or the weight (top-p) of the keys at or above it reaches its share, and how many of the logits equal
 // to it, by index, still belong.
 //
-// A row takes as few passes as its settings allow (one of up to 32768 tokens stays in registers); the first finds the largest logit.
+// A row takes as few passes as its settings allow; the first finds the largest logit.
 //   * Where a bound leaves at most kCap tokens (top-k: the k-th largest of 2048 groups' maxima, four a thread, is no larger than the
 //     k-th largest logit; min-p alone: its logit; or a short row), a second pass gathers them into LDS, 16 a thread, and the
 //     rest works on these.
@@ -28,9 +28,8 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kPer = 16, kCap = kPer * kThreads;  // gathered tokens
+constexpr int kPer = 16, kCap = kPer * kThreads;  // gathered tokens, kPer * 64 of them by each wave
 constexpr int kCell = 256;                       // tokens that a wave takes at once: 4 a lane, side by side
-constexpr int kHeld = 16;                        // cells per wave of a row in registers: 32768 tokens
 constexpr int kAhead = 16;                       // cells per wave whose loads are on the way at once: 128 KB per block
 constexpr int kBinPer = kBins / kThreads;
 constexpr int kGroupMaxK = 1600;                 // top-k that the maxima of 2048 groups bound well
@@ -44,7 +43,7 @@ struct Args {
   const float* u;
   int32_t* ids;
   float* probs;
-  double one;      // 2^s of the comment above, s <= 51
+  int bits;        // s of the comment above, at most 51
   int cell_shift;  // the last pass sums cells of kCell << cell_shift tokens, at most kBins of them
 };
 
@@ -69,16 +68,16 @@ struct Shared {
   };
   u64 wave[kWaves], meta[kWaves];
   u64 got[3];
-  uint32_t count;
+  uint32_t counts[kWaves];  // gathered tokens of each wave
 };
 
-// The row's logits, -inf past its end. ALIGNED: every lane's 4 tokens can be loaded at once. HELD: kept in registers, loaded once. (Passes compare
-// logits, not keys: 2 instructions a token where the keys took 13, and a pass over 131072 tokens 11 us of nothing else. NaN compares false.)
-template <int T, bool ALIGNED, bool HELD>
+// The row's logits, -inf past its end. ALIGNED: every lane's 4 tokens can be loaded at once. (Passes compare logits, not keys: 2
+// instructions a token where the keys took 13, and a pass over 131072 tokens 11 us of nothing else. NaN compares false. Every pass loads
+// them again: kept in registers, a row of 32000 left too few for the weights, 52 us against 46.)
+template <int T, bool ALIGNED>
 struct Row {
   const char* p;
   int V;
-  float z[HELD ? kHeld : 1][4];
 
   __device__ __forceinline__ void load(int at, float (&z)[4]) const {
     constexpr int size = T == EMBER_TYPE_F32 ? 4 : 2;
@@ -108,20 +107,9 @@ struct Row {
     }
   }
   static __device__ int first() { return (int)(threadIdx.x >> 6) * kCell + (int)(threadIdx.x & 63) * 4; }
-  __device__ __forceinline__ void hold() {
-    if constexpr (HELD) {
-#pragma unroll
-      for (int c = 0; c < kHeld; ++c) load(first() + c * kWaves * kCell, z[c]);
-    }
-  }
   // f(index of the first, logits) for this thread's tokens, 4 at a time; whole waves together.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    if constexpr (HELD) {
-#pragma unroll
-      for (int c = 0; c < kHeld; ++c)
-        if (c * kWaves * kCell < V) f(first() + c * kWaves * kCell, z[c]);
-    } else {
       for (int c0 = 0; c0 < V; c0 += kAhead * kWaves * kCell) {
         float x[kAhead][4];
 #pragma unroll
@@ -130,7 +118,6 @@ struct Row {
         for (int c = 0; c < kAhead; ++c)
           if (c0 + c * kWaves * kCell < V) f(first() + c0 + c * kWaves * kCell, x[c]);
       }
-    }
   }
 };
 
@@ -213,27 +200,52 @@ __device__ __forceinline__ void find_bin(Shared& sh, u64* bins, int n, bool down
   __syncthreads();
 }
 
+// exp((z - top) / temperature), as p 2^n: 2^f for the fraction f, by its Taylor series to the 11th power (at |f| <= 1/2 the rest is under 2^-47),
+// some 20 instructions. Infinite logits count as 2^200, which is as far from every finite one as it takes.
 struct Weigh {
   float top;
-  double inv_t, one;
-  __device__ __forceinline__ double e(uint32_t key) const { return at(value_of(key)); }
-  __device__ __forceinline__ double at(float z) const {
-    return z == top ? 1.0 : exp(((double)z - (double)top) * inv_t);
+  double far, c;  // min(top, 2^200); log2(e) / temperature
+  int s;          // weights are summed as integers, times 2^s
+  __device__ __forceinline__ double part(float z, int& n) const {
+    const double y = (fmin((double)z, 0x1p200) - far) * c, r = rint(y), f = y - r;
+    n = (int)fmax(r, -100000.0);
+    double p = 4.44553827187081e-10;
+    p = __builtin_fma(p, f, 7.054911620801121e-09);
+    p = __builtin_fma(p, f, 1.0178086009239696e-07);
+    p = __builtin_fma(p, f, 1.3215486790144305e-06);
+    p = __builtin_fma(p, f, 1.5252733804059838e-05);
+    p = __builtin_fma(p, f, 0.00015403530393381606);
+    p = __builtin_fma(p, f, 0.0013333558146428441);
+    p = __builtin_fma(p, f, 0.009618129107628477);
+    p = __builtin_fma(p, f, 0.055504108664821576);
+    p = __builtin_fma(p, f, 0.2402265069591007);
+    p = __builtin_fma(p, f, 0.6931471805599453);
+    return __builtin_fma(p, f, 1.0);
+  }
+  __device__ __forceinline__ double e(uint32_t key) const {
+    int n;
+    const double p = part(value_of(key), n);
+    return ldexp(p, n);
   }
   // e 2^s to the nearest integer: the low bits of 2^52 plus it
-  __device__ __forceinline__ u64 fix(double e) const { return __double_as_longlong(__builtin_fma(e, one, 0x1p52)) - __double_as_longlong(0x1p52); }
+  __device__ __forceinline__ u64 fix(double e) const { return __double_as_longlong(ldexp(e, s) + 0x1p52) - __double_as_longlong(0x1p52); }
+  __device__ __forceinline__ u64 at(float z) const {
+    int n;
+    const double p = part(z, n);
+    return __double_as_longlong(ldexp(p, n + s) + 0x1p52) - __double_as_longlong(0x1p52);
+  }
 };
 
-// Over the threads' items (amount a[i], 0: none): the largest key t in [lo, hi] whose keys >= t hold `need` together with `above`, which
+// Over the threads' items (the first n, the same for a wave; amount a[i], 0: none): the largest key t in [lo, hi] whose keys >= t hold `need` together with `above`, which
 // gets what the keys > t hold. Eleven bits of the difference to lo at a time.
 template <int N>
-__device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&key)[N], const u64 (&a)[N], uint32_t lo, uint32_t hi, u64 need, u64& above) {
+__device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&key)[N], const u64 (&a)[N], int n, uint32_t lo, uint32_t hi, u64 need, u64& above) {
   uint32_t width = hi - lo;
   int s = max(0, 32 - __clz((int)width) - 11);
   for (;;) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (a[i] && key[i] - lo <= width) atomicAdd(&sh.bin[(key[i] - lo) >> s], a[i]);  // (a key under lo is far above width)
+      if (i < n && a[i] && key[i] - lo <= width) atomicAdd(&sh.bin[(key[i] - lo) >> s], a[i]);  // (a key under lo is far above width)
     __syncthreads();
     find_bin(sh, sh.bin, kBins, true, above, need);
     lo += (uint32_t)sh.got[0] << s;
@@ -244,37 +256,44 @@ __device__ __forceinline__ uint32_t select_items(Shared& sh, const uint32_t (&ke
   }
 }
 
-// Gathers the tokens that `is` picks (by their logit; none that is never drawn), in any order; whether they fit.
+// Gathers the tokens that `is` picks (by their logit; none that is never drawn), each wave those of its cells, in any order; whether they fit.
+// (A list for all, its places given out by an atomic, had every wave wait for LDS at each cell: 9 us of 42 for a row of 32000.)
 template <class R, class F>
 __device__ __forceinline__ bool gather(const R& r, Shared& sh, F is) {
-  if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
+  const int wave = threadIdx.x >> 6, base = wave * kPer * 64;
+  uint32_t count = 0;  // the wave's
   r.each([&](int i, const float (&z)[4]) {
-    uint32_t n = 0;
-    bool in[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) in[e] = is(z[e]);
-    if (!__ballot(in[0] || in[1] || in[2] || in[3])) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) n += in[e];
-    const uint32_t upto = wave_upto(n);
-    uint32_t at = 0;
-    if ((threadIdx.x & 63) == 63) at = atomicAdd(&sh.count, upto);
-    at = last_lane(at) + upto - n;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (in[e]) {
-        if (at < kCap) {
-          sh.key[at] = key_of(z[e]);
-          sh.idx[at] = (uint32_t)(i + e);
-        }
-        ++at;
+    for (int e = 0; e < 4; ++e) {
+      const bool in = is(z[e]);
+      const u64 mask = __ballot(in);
+      if (!mask) continue;
+      const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      if (in && at < kPer * 64) {
+        sh.key[base + at] = key_of(z[e]);
+        sh.idx[base + at] = (uint32_t)(i + e);
       }
+      count += (uint32_t)__popcll(mask);
+    }
   });
+  if ((threadIdx.x & 63) == 0) sh.counts[wave] = count;
   __syncthreads();
-  const bool fits = sh.count <= kCap;
+  bool fits = true;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) fits &= sh.counts[v] <= kPer * 64;
   __syncthreads();
   return fits;
+}
+// This thread's gathered item i, whether there is one; the wave's number of items per thread.
+__device__ __forceinline__ bool item(const Shared& sh, int i, uint32_t& key, uint32_t& idx) {
+  const int wave = threadIdx.x >> 6, at = i * 64 + (int)(threadIdx.x & 63);
+  if (at >= (int)sh.counts[wave]) return false;
+  key = sh.key[wave * kPer * 64 + at];
+  idx = sh.idx[wave * kPer * 64 + at];
+  return true;
+}
+__device__ __forceinline__ int items(const Shared& sh) {
+  return (__builtin_amdgcn_readfirstlane((int)sh.counts[threadIdx.x >> 6]) + 63) / 64;
 }
 
 // select_items over the whole row by the key's digits, for the keys above floor_key and `extra` for that key itself. MASS: by weight.
@@ -287,7 +306,7 @@ __device__ __forceinline__ uint32_t select_row(const R& r, Shared& sh, const Wei
     r.each([&](int, const float (&z)[4]) {
       for (int e = 0; e < 4; ++e) {
         const uint32_t k = key_of(z[e]);
-        if (k > floor_key && (!p || (k >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(k >> s) & (nb - 1)], MASS ? w.fix(w.at(z[e])) : 1ull);
+        if (k > floor_key && (!p || (k >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(k >> s) & (nb - 1)], MASS ? w.at(z[e]) : 1ull);
       }
     });
     if (extra && threadIdx.x == 0 && (!p || (floor_key >> (s + bits)) == prefix)) atomicAdd(&sh.bin[(floor_key >> s) & (nb - 1)], extra);
@@ -323,7 +342,7 @@ __device__ __forceinline__ void bins_row(const R& r, Shared& sh, const Weigh& w,
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (z[e] > above) {
-        const u64 x = MASS ? w.fix(w.at(z[e])) : 1ull;
+        const u64 x = MASS ? w.at(z[e]) : 1ull;
         if (x) atomicAdd(&sh.bin[bin_of(z[e])], x);
         sum += x;
       }
@@ -342,13 +361,17 @@ __device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const 
   if (!gather(r, sh, [&](float z) { return z > under && bin_of(z) == b; })) return select_row<MASS>(r, sh, w, floor_key, extra, need, above);
   uint32_t key[kPer], lo = ~0u, hi = 0;
   u64 x[kPer], here = 0;
+  const int n = items(sh);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const uint32_t at = i * kThreads + threadIdx.x;
-    key[i] = at < sh.count ? sh.key[at] : 0;
-    x[i] = !key[i] ? 0 : MASS ? w.fix(w.e(key[i])) : 1ull;
-    here += x[i];
-    if (key[i]) lo = min(lo, key[i]), hi = max(hi, key[i]);
+    uint32_t idx;
+    key[i] = 0;
+    x[i] = 0;
+    if (i < n && item(sh, i, key[i], idx)) {
+      x[i] = MASS ? w.fix(w.e(key[i])) : 1ull;
+      here += x[i];
+      lo = min(lo, key[i]), hi = max(hi, key[i]);
+    }
   }
   if (extra) {  // should the bin's tokens not reach `need`, it is the floor key, in the same bin, that does
     here = block_sum(sh, here);
@@ -367,10 +390,10 @@ __device__ __forceinline__ uint32_t threshold_row(const R& r, Shared& sh, const 
     hi = max(hi, (uint32_t)(sh.wave[v] >> 32));
   }
   __syncthreads();
-  return select_items(sh, key, x, lo, hi, need, above);
+  return select_items(sh, key, x, n, lo, hi, need, above);
 }
 
-template <int T, bool ALIGNED, bool HELD>
+template <int T, bool ALIGNED>
 __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   Shared& sh = *reinterpret_cast<Shared*>(lds);
@@ -386,10 +409,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   min_p = fminf(min_p, 1.0f);
   float u = a.u[row];
   u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-  Row<T, ALIGNED, HELD> r;
+  Row<T, ALIGNED> r;
   r.p = static_cast<const char*>(a.z) + row * a.stride * (T == EMBER_TYPE_F32 ? 4 : 2);
   r.V = a.V;
-  r.hold();
 
   // the largest logit of the row and of this thread's four groups, which four tokens first held its largest, how many can be drawn
 #pragma unroll
@@ -438,7 +460,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     }
     return;
   }
-  const Weigh w{value_of(top_key), 1.0 / (double)temp, a.one};
+  const float top = value_of(top_key);
+  const Weigh w{top, fmin((double)top, 0x1p200), top > 3.4028235e38f ? 1.0 : 1.4426950408889634074 / (double)temp, a.bits};
   bool by_k = top_k > 0 && (uint32_t)top_k < n_valid, by_p = top_p < 1.0f;
 
   // a key that no token to be kept is under: `low` of all, `floor` (0: none) where few tokens are at or above it
@@ -454,7 +477,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = group_key[e] != 0;
     u64 above = 0;
-    if (block_sum(sh, x[0] + x[1] + x[2] + x[3]) >= (u64)top_k) low = floor = select_items(sh, group_key, x, max(least, 1u), top_key, (u64)top_k, above);
+    if (block_sum(sh, x[0] + x[1] + x[2] + x[3]) >= (u64)top_k) low = floor = select_items(sh, group_key, x, 4, max(least, 1u), top_key, (u64)top_k, above);
   }
   auto from = [](float bound) { return [bound](float z) { return z >= bound; }; };
   // (key 1 is a NaN's neighbour: the lowest logit that can be drawn)
@@ -505,26 +528,29 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
   if (listed) {
     uint32_t key[kPer], idx[kPer];  // idx: inverted, so that the first index is the largest
     u64 x[kPer];
-    const uint32_t n = sh.count, inv_lo = ~(uint32_t)(a.V - 1);
+    const uint32_t inv_lo = ~(uint32_t)(a.V - 1);
+    const int n = items(sh);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t at = i * kThreads + tid;
-      key[i] = at < n ? sh.key[at] : 0;
-      idx[i] = at < n ? ~sh.idx[at] : 0;
-      x[i] = key[i] != 0;
+      key[i] = 0;
+      idx[i] = ~0u;
+      x[i] = i < n && item(sh, i, key[i], idx[i]);
+      idx[i] = ~idx[i];
     }
     // keeps of the items equal to t the first `keep` by index, and none under it
     auto cut = [&](uint32_t t_, u64 keep) {
       u64 eq[kPer], mine = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
+        eq[i] = 0;
+        if (i >= n) continue;
         if (key[i] < t_) x[i] = 0;
         eq[i] = x[i] && key[i] == t_;
         mine += eq[i];
       }
       if (block_sum(sh, mine) <= keep) return;
       u64 before = 0;
-      const uint32_t last = select_items(sh, idx, eq, inv_lo, ~0u, keep, before);
+      const uint32_t last = select_items(sh, idx, eq, n, inv_lo, ~0u, keep, before);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (eq[i] && idx[i] < last) x[i] = 0;
@@ -532,13 +558,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     if (t) cut(t, ties);
     if (by_k) {
       u64 above = 0;
-      const uint32_t t_ = select_items(sh, key, x, low, top_key, (u64)top_k, above);
+      const uint32_t t_ = select_items(sh, key, x, n, low, top_key, (u64)top_k, above);
       cut(t_, (u64)top_k - above);
     }
     uint32_t under = 0;  // bit i: item i has less than min_p
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      if (x[i]) {
+      if (i < n && x[i]) {
         const double e = w.e(key[i]);
         x[i] = w.fix(e);
         under |= (uint32_t)(e < (double)min_p) << i;
@@ -548,7 +574,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) mine += x[i];
       const u64 need = need_p ? need_p : max(1ull, (u64)ceil((double)top_p * (double)block_sum(sh, mine)));
-      const uint32_t t_ = select_items(sh, key, x, low, top_key, need, above);
+      const uint32_t t_ = select_items(sh, key, x, n, low, top_key, need, above);
       const u64 each_ = w.fix(w.e(t_));
       cut(t_, (need - above + each_ - 1) / each_);
     }
@@ -560,7 +586,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     }
     const u64 sum = block_sum(sh, mine), target = (u64)((double)u * (double)sum);
     u64 before = 0;
-    const uint32_t drawn = select_items(sh, idx, x, inv_lo, ~0u, target + 1, before);
+    const uint32_t drawn = select_items(sh, idx, x, n, inv_lo, ~0u, target + 1, before);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (x[i] && idx[i] == drawn) {
@@ -572,7 +598,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 
   // Too many to gather: the weights of the tokens above t, and the tokens equal to it, by cells of consecutive tokens, a wave a cell.
   auto weight = [&](float z) -> u64 {
-    const double e = w.at(z);
+    const double e = w.e(key_of(z));
     return e >= (double)min_p ? w.fix(e) : 0;
   };
   const float tz = t ? value_of(t) : -INFINITY;
@@ -665,9 +691,7 @@ int launch(const Args& a, int n, bool aligned, hipStream_t st) {
     kernel<<<n, kThreads, sizeof(Shared), st>>>(a);
     return hipGetLastError() == hipSuccess ? (int)EMBER_OK : (int)EMBER_ERR_LAUNCH;
   };
-  const bool held = a.V <= kHeld * kWaves * kCell;
-  if (aligned) return held ? go(sample_kernel<T, true, true>) : go(sample_kernel<T, true, false>);
-  return held ? go(sample_kernel<T, false, true>) : go(sample_kernel<T, false, false>);
+  return aligned ? go(sample_kernel<T, true>) : go(sample_kernel<T, false>);
 }
 
 }  // namespace
@@ -687,8 +711,8 @@ extern "C" int ember_sample(const ember_sampler* s, const void* logits, int type
   int bits = 0, shift = 0;
   while ((1 << bits) < V) ++bits;
   while (((V + (kCell << shift) - 1) / (kCell << shift)) > kBins) ++shift;
-  const Args a{*s, logits, V, stride, u, ids, probs, (double)(1ull << std::min(51, 61 - bits)), shift};
   const bool aligned = !off(logits, 4 * size) && (n == 1 || stride % 4 == 0);
+  const Args a{*s, logits, V, stride, u, ids, probs, std::min(51, 61 - bits), shift};
   switch (type) {
     case EMBER_TYPE_F32: return launch<EMBER_TYPE_F32>(a, n, aligned, stream);
     case EMBER_TYPE_F16: return launch<EMBER_TYPE_F16>(a, n, aligned, stream);
