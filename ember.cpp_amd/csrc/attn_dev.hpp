@@ -67,6 +67,22 @@ __device__ inline s8 codes_times(u2 w, h8 s) {
   return __builtin_bit_cast(s8, __builtin_bit_cast(h8, c) * s);
 }
 
+// 16 bytes per lane from global memory into LDS, lane after lane from `lds` on, without registers.
+__device__ inline void load_to_lds(const void* g, char* lds) {
+  __builtin_amdgcn_global_load_lds(g, (EMBER_LDS(void)*)lds, 16, 0, 0);
+}
+// All of this wave's loads, to registers and to LDS, have arrived; all its LDS reads are done.
+__device__ inline void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+__device__ inline void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
 // Whether one of 8 halves is infinite or NaN.
 template <bool BF16>
 __device__ inline bool not_finite(u4 v) {

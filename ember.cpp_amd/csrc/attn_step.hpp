@@ -45,22 +45,6 @@ __device__ inline RowScales<KS> row_scales(const _Float16* p, uint32_t row, int 
   }
 }
 
-// 16 bytes per lane from global memory into LDS, lane after lane from `lds` on, without registers.
-__device__ inline void load_to_lds(const void* g, char* lds) {
-  __builtin_amdgcn_global_load_lds(g, (EMBER_LDS(void)*)lds, 16, 0, 0);
-}
-// All of this wave's loads, to registers and to LDS, have arrived; all its LDS reads are done.
-__device__ inline void wait_loads() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  asm volatile("" ::: "memory");
-}
-__device__ inline void wait_lds() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-}
-
 // EXACT: rows of DP columns, not fewer.
 template <int T, int IO, int DP, bool GEN, bool EXACT>
 __global__ __launch_bounds__(kStepThreads, DP > 128 ? (Op<T>::kQ8 ? 2 : 1) : Op<T>::kQ8 ? 3 : 2) void attn_step_kernel(AttnArgs a, Parts parts, int part0, int tiles, int chunk, int begin) {

@@ -2,9 +2,9 @@
 // attn_wide_*.hip.
 //
 // Bound by the matrix cores. A block takes 128 query rows of one KV head (the heads that share it are rows too, so their keys
-// are loaded once), 32 for each of its four waves, and goes through the keys in tiles that all waves read from LDS. The next tile's
-// rows are loaded into registers while this one is computed, and stored to the other half of the LDS (quantised rows as fp16:
-// converted once for all four waves); one barrier per tile. 32 x 32 x 16 products: a lane holds half of the scores of one query row.
+// are loaded once), 32 for each of its four waves, and goes through the keys in tiles that all waves read from LDS. The next tile
+// comes into the other half of the LDS while this one is computed: rows of halves straight, quantised rows by way of
+// registers, as fp16 (converted once for all four waves); one barrier per tile. 32 x 32 x 16 products: a lane holds half of the scores of one query row.
 #pragma once
 #include "attn_dev.hpp"
 
@@ -39,9 +39,9 @@ __device__ inline int seq_of(const CacheArgs& c, int i) {
   return lo;
 }
 
-// SHARED: the rows are those of the whole batch, the keys the first `end` of sequence 0's. Otherwise blockIdx.y is the sequence, and
+// EXACT: rows of DP columns, not fewer. SHARED: the rows are those of the whole batch, the keys the first `end` of sequence 0's. Otherwise blockIdx.y is the sequence, and
 // keys before `begin` are left out.
-template <int T, int IO, int DP, bool GEN, bool SHARED>
+template <int T, int IO, int DP, bool GEN, bool SHARED, bool EXACT>
 __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_kernel(AttnArgs a, Parts parts, int part0, int tiles, int splits,
                                                                                  int chunk, int begin, int end) {
   using O = Op<T>;
@@ -155,91 +155,125 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
   for (int d = 0; d < DT; ++d)
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
-  // loads: row tid / CH (+ RPI i) of a tile, chunk tid % CH: 8 values, 16 bytes of halves or 8 codes
+  // Loads: row tid / CH (+ RPI i) of a tile, a chunk of 8 values: 16 bytes of halves or 8 codes. DMA: the 16 bytes at 16 tid (+ 4096 i) of the
+  // stage's K and V, which hold the chunks that k_at and v_at put there.
+  constexpr bool DMA = !O::kQ8 && EXACT;
   const int l_row = tid / CH, l_ch = tid % CH;
-  const bool l_in = l_ch * 8 < c.D;
   const bool whole = !c.pages || c.page.d % KT == 0;  // a tile lies in one page
-  u4 kr[NL], vr[NL];
+  u4 kr[DMA ? 1 : NL], vr[DMA ? 1 : NL];
   uint32_t ks_[NL], vs_[NL];  // Q8_0: the scales' bits
   uint32_t torn = 0;          // bit i: this thread's row i is in no page
-  auto load = [&](int kt) {
-    uint32_t base = 0;
-    if (whole) {
-      const int64_t rr = cache_row(c, kv_seq, kt);
-      base = rr < 0 ? ~0u : (uint32_t)(rr + (int64_t)kvh * c.page.d);
-    }
-    torn = 0;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int j = min(kt + l_row + i * RPI, hi - 1);
-      uint32_t row;
-      if (whole) {
-        row = base == ~0u ? ~0u : base + (uint32_t)(j - kt);
+  auto row_at = [&](int j) -> uint32_t {
+    const int64_t rr = cache_row(c, kv_seq, j);
+    return rr < 0 ? ~0u : (uint32_t)(rr + (int64_t)kvh * c.page.d);
+  };
+  // chunk of row `row` that is loaded for place (key, l_ch)
+  auto k_chunk = [&](int key) { return DMA ? (k_at<CH>(key, l_ch) >> 4) % CH : l_ch; };
+  auto v_chunk = [&](int key) { return DMA ? (v_at<CH, false>(key, l_ch) >> 4) % CH : l_ch; };
+  auto load_row = [&](int i, const char* k, const char* v, int64_t k_off, int64_t v_off, int64_t s_off, int stage) {
+    if constexpr (DMA) {
+      char* const to = lds + stage * L::kStage + (i * kWideThreads + wave * 64) * 16;
+      load_to_lds(k + k_off, to);
+      load_to_lds(v + v_off, to + L::kTile);
+    } else if (EXACT || l_ch * 8 < c.D) {
+      if constexpr (O::kQ8) {
+        const u2 kk = *reinterpret_cast<const u2*>(k + k_off), vv = *reinterpret_cast<const u2*>(v + v_off);
+        kr[i] = u4{kk[0], kk[1], 0, 0};
+        vr[i] = u4{vv[0], vv[1], 0, 0};
+        ks_[i] = __builtin_bit_cast(uint16_t, c.ks[s_off]);
+        vs_[i] = __builtin_bit_cast(uint16_t, c.vs[s_off]);
       } else {
-        const int64_t rr = cache_row(c, kv_seq, j);
-        row = rr < 0 ? ~0u : (uint32_t)(rr + (int64_t)kvh * c.page.d);
+        kr[i] = *reinterpret_cast<const u4*>(k + k_off);
+        vr[i] = *reinterpret_cast<const u4*>(v + v_off);
       }
-      if (row == ~0u) {
-        torn |= 1u << i;
-        row = 0;
-      }
-      const int64_t at = ((int64_t)row * c.D + l_ch * 8) * O::kBytes;
+    } else {
       kr[i] = vr[i] = u4{0, 0, 0, 0};
       ks_[i] = vs_[i] = 0;
-      if (l_in) {
-        if constexpr (O::kQ8) {
-          const u2 kk = *reinterpret_cast<const u2*>(static_cast<const char*>(c.k) + at), vv = *reinterpret_cast<const u2*>(static_cast<const char*>(c.v) + at);
-          kr[i] = u4{kk[0], kk[1], 0, 0};
-          vr[i] = u4{vv[0], vv[1], 0, 0};
-          const int64_t sat = (int64_t)row * (c.D / 32) + l_ch / 4;
-          ks_[i] = __builtin_bit_cast(uint16_t, c.ks[sat]);
-          vs_[i] = __builtin_bit_cast(uint16_t, c.vs[sat]);
-        } else {
-          kr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.k) + at);
-          vr[i] = *reinterpret_cast<const u4*>(static_cast<const char*>(c.v) + at);
+    }
+  };
+  auto load = [&](int kt, int stage) {
+    const int64_t row_bytes = (int64_t)(EXACT ? DP : c.D) * O::kBytes;
+    const int nb = (EXACT ? DP : c.D) / 32;
+    const char *const ck = static_cast<const char*>(c.k), *const cv = static_cast<const char*>(c.v);
+    const uint32_t base = whole ? row_at(kt) : 0;
+    torn = 0;
+    if (whole && kt + KT <= hi && base != ~0u) {  // the plain case: rows of one page, one after the other
+      const char *const k = ck + base * row_bytes, *const v = cv + base * row_bytes;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int key = l_row + i * RPI, at = key * (int)row_bytes;
+        load_row(i, k, v, at + k_chunk(key) * 8 * O::kBytes, at + v_chunk(key) * 8 * O::kBytes, (int64_t)base * nb + key * nb + l_ch / 4, stage);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int key = l_row + i * RPI, j = min(kt + key, hi - 1);
+        uint32_t row = !whole ? row_at(j) : base == ~0u ? base : base + (uint32_t)(j - kt);
+        if (row == ~0u) {
+          torn |= 1u << i;
+          row = 0;
         }
+        load_row(i, ck, cv, row * row_bytes + k_chunk(key) * 8 * O::kBytes, row * row_bytes + v_chunk(key) * 8 * O::kBytes, (int64_t)row * nb + l_ch / 4, stage);
       }
     }
   };
-  // into stage s; values of keys that the block does not see as zeros. A tile that some rows see in part only (`part`) must not
-  // hold values that are not finite, since a weight of 0 times one is NaN: they are stored as zeros too, and their key is noted
-  auto store = [&](int kt, int s, bool part, unsigned long long* odd) {
-    char* const kl = lds + s * L::kStage;
+  // Into the stage, if it is not there yet; values of keys that the block does not see as zeros. A tile that some rows see in part only
+  // (`part`) must not hold values that are not finite, since a weight of 0 times one is NaN: they become zeros too, and their key is noted. A key
+  // in no page becomes NaN, which makes its scores so.
+  auto store = [&](int kt, int stage, bool part, unsigned long long* odd) {
+    char* const kl = lds + stage * L::kStage;
     char* const vl = kl + L::kTile;
-    const bool inside = kt >= lo && kt + KT <= hi;
+    const u4 nan = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}, zero = {0, 0, 0, 0};
+    if constexpr (DMA) {
+      wait_loads();
+      if (!part && torn == 0) return;
+    }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int key = l_row + i * RPI;
-      u4 kk = kr[i], vv = vr[i];
-      if constexpr (O::kQ8) {
-        auto held = [](u4 w, uint32_t bits) {
-          const _Float16 s_ = __builtin_bit_cast(_Float16, (uint16_t)bits);
-          return __builtin_bit_cast(u4, codes_times(u2{w[0], w[1]}, h8{s_, s_, s_, s_, s_, s_, s_, s_}));
-        };
-        kk = held(kk, ks_[i]);
-        vv = held(vv, vs_[i]);
+      if constexpr (DMA) {
+        char* const to = kl + (i * kWideThreads + tid) * 16;
+        u4 vv = *reinterpret_cast<const u4*>(to + L::kTile);
+        bool put = kt + key < lo || kt + key >= hi;
+        if (!put && not_finite<O::kBf16>(vv)) {
+          put = true;
+          atomicOr(odd, 1ull << key);
+        }
+        if (put) *reinterpret_cast<u4*>(to + L::kTile) = zero;
+        if (torn >> i & 1) *reinterpret_cast<u4*>(to) = nan;
+      } else {
+        u4 kk = kr[i], vv = vr[i];
+        if constexpr (O::kQ8) {
+          auto held = [](u4 w, uint32_t bits) {
+            const _Float16 s_ = __builtin_bit_cast(_Float16, (uint16_t)bits);
+            return __builtin_bit_cast(u4, codes_times(u2{w[0], w[1]}, h8{s_, s_, s_, s_, s_, s_, s_, s_}));
+          };
+          kk = held(kk, ks_[i]);
+          vv = held(vv, vs_[i]);
+        }
+        if (part) {
+          if (kt + key < lo || kt + key >= hi) vv = zero;
+          if (not_finite<O::kBf16>(vv)) {
+            vv = zero;
+            atomicOr(odd, 1ull << key);
+          }
+        }
+        if (torn >> i & 1) kk = nan;
+        *reinterpret_cast<u4*>(kl + k_at<CH>(key, l_ch)) = kk;
+        *reinterpret_cast<u4*>(vl + v_at<CH, false>(key, l_ch)) = vv;
       }
-      if (!inside && (kt + key < lo || kt + key >= hi)) vv = u4{0, 0, 0, 0};
-      // a key in no page: NaN, which makes its scores so
-      if (torn >> i & 1) kk = u4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
-      if (part && not_finite<O::kBf16>(vv)) {
-        vv = u4{0, 0, 0, 0};
-        atomicOr(odd, 1ull << key);
-      }
-      *reinterpret_cast<u4*>(kl + k_at<CH>(key, l_ch)) = kk;
-      *reinterpret_cast<u4*>(vl + v_at<CH, false>(key, l_ch)) = vv;
     }
   };
   auto in_part = [&](int kt) { return kt < b_lo || kt + KT > b_hi; };
 
   if (k0 < k1) {
-    load(k0);
+    load(k0, 0);
     store(k0, 0, in_part(k0), &odd_keys[0]);
     __syncthreads();
   }
   for (int kt = k0, n = 0; kt < k1; kt += KT, ++n) {
     const bool more = kt + KT < k1;
-    if (more) load(kt + KT);
+    if (more) load(kt + KT, (n + 1) & 1);
     if (tid == 0) odd_keys[(n + 2) & 3] = 0;  // (two barriers after it was read, one before it is written again)
     if (kt < w_hi && kt + KT > w_lo) {
       const char* const kl = lds + (n & 1) * L::kStage;
@@ -353,10 +387,10 @@ int launch_wide(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_
   const dim3 grid((unsigned)(tiles * w.splits * a.c.n_kv), SHARED ? 1 : a.c.n_seqs);
   constexpr size_t lds = WideLds<DP>::kBytes;
   static_assert(lds <= 65536, "no attribute needed");
-  if (a.softcap > 0.0f || a.slopes)
-    attn_wide_kernel<T, IO, DP, true, SHARED><<<grid, kWideThreads, lds, st>>>(a, p, w.part0, (int)tiles, w.splits, w.chunk, w.begin, w.end);
-  else
-    attn_wide_kernel<T, IO, DP, false, SHARED><<<grid, kWideThreads, lds, st>>>(a, p, w.part0, (int)tiles, w.splits, w.chunk, w.begin, w.end);
+  auto go = [&](auto* kernel) { kernel<<<grid, kWideThreads, lds, st>>>(a, p, w.part0, (int)tiles, w.splits, w.chunk, w.begin, w.end); };
+  const bool gen = a.softcap > 0.0f || a.slopes;
+  if (a.c.D == DP) gen ? go(attn_wide_kernel<T, IO, DP, true, SHARED, true>) : go(attn_wide_kernel<T, IO, DP, false, SHARED, true>);
+  else gen ? go(attn_wide_kernel<T, IO, DP, true, SHARED, false>) : go(attn_wide_kernel<T, IO, DP, false, SHARED, false>);
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }
 
