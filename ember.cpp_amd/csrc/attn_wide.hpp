@@ -27,6 +27,20 @@ struct WideLds {
   static constexpr int kBytes = 2 * kStage;
 };
 
+// Asks the scheduler for N products, each fed by R reads from LDS, with the reads of AHEAD products on the way before the first: left to
+// itself, short of registers, it waits for every read in turn.
+template <int N, int R, int AHEAD>
+__device__ __forceinline__ void lds_ahead() {
+  constexpr int A = AHEAD < N ? AHEAD : N;
+  __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);
+#pragma unroll
+  for (int i = 0; i < N - A; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x8, A, 0);
+}
+
 // The sequence of row i of the batch, n_seqs for rows of none.
 __device__ inline int seq_of(const CacheArgs& c, int i) {
   if (!c.q_start) return i;
@@ -271,6 +285,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
     store(k0, 0, in_part(k0), &odd_keys[0]);
     __syncthreads();
   }
+  wait_loads();  // (the query's too, on every path into the loop: else the first product of each tile waits for all loads)
   for (int kt = k0, n = 0; kt < k1; kt += KT, ++n) {
     const bool more = kt + KT < k1;
     if (more) load(kt + KT, (n + 1) & 1);
@@ -288,6 +303,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
           s[u] = mma32<O::kBf16>(kf, qf[q], s[u]);
         }
       }
+      lds_ahead<NS * KS, 1, 6>();
       // key of score i of half-tile u: 8 (i / 4) + 4 half + i % 4
       const bool masked = kt < all_lo || kt + KT > all_hi;
       if (GEN) {
@@ -347,6 +363,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
           const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((EMBER_LDS(s4)*)(vl + v_at<CH, false>(16 * q + 8 + v_key, 4 * d + v_c) + (lane & 1) * 8));
           o[d] = mma32<O::kBf16>(s8{y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]}, pf[q], o[d]);
         }
+      lds_ahead<NS * 2 * DT, 2, 4>();
     }
     if (more) store(kt + KT, (n + 1) & 1, in_part(kt + KT), &odd_keys[(n + 1) & 3]);
     __syncthreads();
