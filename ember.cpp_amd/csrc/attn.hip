@@ -6,35 +6,42 @@
 namespace ember_attn_impl {
 namespace {
 
-// Rows of parts (Parts) as output rows: a block per row, four waves on a quarter of the parts each. A wave's lanes first hold one
-// part's maximum and sum each, then the row's columns. (A wave alone took 126 us for 32 rows of 256 parts: one load after another.)
-template <int IO>
+// Rows of parts (Parts) as output rows: W waves of a block per row, each on a share of the parts, four rows or one per block. A wave's
+// lanes first hold one part's maximum and sum each, then the row's columns. W = 4 where parts are many (a wave alone took 126 us for 32
+// rows of 256 parts: one load after another), 1 where they are few, and rows may be many.
+constexpr int kFewParts = 16;
+template <int IO, int W>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts) {
-  __shared__ f4 xs[4][64];
-  __shared__ float ms[4], sums[4];
+  __shared__ f4 xs[W][64];
+  __shared__ float ms[W], sums[W];
+  constexpr int U = W > 1 ? 2 : 1;  // (at most 512 parts)
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.x / a.H, h = blockIdx.x - tok * a.H;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = W > 1 ? blockIdx.x : blockIdx.x * 4 + wave, tok = at / a.H, h = at - tok * a.H;
   int first, count;
   seq_rows(c, blockIdx.y, first, count);
   if (tok >= min(count, c.max_q)) return;
   const int64_t row = (int64_t)(first + tok) * a.H + h;
-  const int per = (parts.n + 3) / 4, from = wave * per, n = min(per, parts.n - from);  // (at most 128 parts a wave)
+  const int per = (parts.n + W - 1) / W, from = W > 1 ? wave * per : 0, n = min(per, parts.n - from);
   const int d = min(lane * 4, c.D - 4);
-  float m[2] = {kNoScore, kNoScore}, l[2] = {0.0f, 0.0f};
+  float m[U], l[U], M = kNoScore;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < U; ++u) {
+    m[u] = kNoScore;
+    l[u] = 0.0f;
     if (u * 64 + lane < n) {
       const float* ml = parts.ml + ((from + u * 64 + lane) * parts.rows + row) * 2;
       m[u] = ml[0];
       l[u] = ml[1];
     }
-  float M = fmaxf(m[0], m[1]);
-  for (int k = 32; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+    M = fmaxf(M, m[u]);
+  }
+  for (int k = W > 1 ? 32 : kFewParts / 2; k; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+  if (W == 1) M = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, M)));
   float sum = 0.0f;
   f4 x = {0, 0, 0, 0};
   const float* const o = parts.o + (from * parts.rows + row) * c.D + d;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < U; ++u) {
     const float w = exp2_fast(m[u] - M);
     sum += l[u] * w;
     const float live = l[u] != 0.0f ? w : -1.0f;  // (parts without a visible key hold nothing; NaN is not 0)
@@ -57,27 +64,41 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts)
     }
   }
   for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-  xs[wave][lane] = x;
-  if (lane == 0) {
-    ms[wave] = M;
-    sums[wave] = sum;
+  if constexpr (W > 1) {
+    xs[wave][lane] = x;
+    if (lane == 0) {
+      ms[wave] = M;
+      sums[wave] = sum;
+    }
+    __syncthreads();
+    if (wave) return;
+    M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+    sum = 0.0f;
+    x = f4{0, 0, 0, 0};
+    for (int w = 0; w < W; ++w) {
+      const float al = exp2_fast(ms[w] - M);
+      sum += sums[w] * al;
+      f4 y = xs[w][lane];
+      y *= al;
+      x += y;
+    }
   }
-  __syncthreads();
-  if (wave || lane * 4 >= c.D) return;
-  M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-  sum = 0.0f;
-  x = f4{0, 0, 0, 0};
-  for (int w = 0; w < 4; ++w) {
-    const float al = exp2_fast(ms[w] - M);
-    sum += sums[w] * al;
-    f4 y = xs[w][lane];
-    y *= al;
-    x += y;
-  }
+  if (lane * 4 >= c.D) return;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   x *= inv;
   const u2 y = {pack2<IO == EMBER_TYPE_BF16>(x[0], x[1]), pack2<IO == EMBER_TYPE_BF16>(x[2], x[3])};
   *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
+}
+
+template <int IO>
+int launch_join(const AttnArgs& a, const Parts& parts, hipStream_t st) {
+  const int64_t rows = (int64_t)a.c.max_q * a.H;
+  const bool few = parts.n <= kFewParts;
+  if (rows > 0x7fffffff) return EMBER_ERR_SHAPE;
+  const dim3 grid((unsigned)(few ? (rows + 3) / 4 : rows), a.c.n_seqs);
+  if (few) attn_join_kernel<IO, 1><<<grid, 256, 0, st>>>(a, parts);
+  else attn_join_kernel<IO, 4><<<grid, 256, 0, st>>>(a, parts);
+  return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -108,8 +129,12 @@ AttnPlan attn_plan(const AttnArgs& a) {
   // 2048 blocks 102 / 108 / 116 us, 8 sequences of up to 20000 Q8_0 tokens on 512 / 768 / 1024 78 / 66 / 77); up to 256 keys in one part,
   // which saves the join (256 keys 9.3 us in one part, 10.7 in two; 512 11.6, 11.0).
   const int places = 256 * (c.D > 128 ? (q8 ? 2 : 1) : q8 ? 3 : 2);
+  // Many rows: two blocks per CU, and parts of 512 keys and more while the join's traffic stays under 32 MB (1024 new tokens of 32 heads in one part / two
+  // 33 / 45 us, 512 20 / 25; 64 after 8000 in 31 parts / 15 / 7 29 / 37 / 60).
+  const int64_t joined = (int64_t)c.n_tokens * a.H * c.D * 8, most = std::max<int64_t>(1, ((int64_t)32 << 20) / std::max<int64_t>(joined, 1));
+  const int64_t wide_blocks = groups * ((rows + 127) / 128);
   if (p.step) split(range, groups * ((rows + 15) / 16), range <= 256 ? 1 : places, 128, p.splits, p.chunk);
-  else split(range, groups * ((rows + 127) / 128), 512, 256, p.splits, p.chunk);
+  else split(range, wide_blocks, std::min<int64_t>(512, most * wide_blocks), 512, p.splits, p.chunk);
   if (p.begin) split(p.begin, c.n_kv * (((int64_t)c.n_tokens * a.G + 127) / 128), 512, 256, p.shared_splits, p.shared_chunk);
   p.parts = p.splits + p.shared_splits > 1 ? p.splits + p.shared_splits : 0;
   return p;
@@ -136,11 +161,7 @@ int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st) {
   if (p.step) s = steps[kind](a, parts, p.shared_splits, p.splits, p.chunk, p.begin, st);
   else s = wides[kind](a, parts, WideCall{p.shared_splits, p.splits, p.chunk, p.begin, 0}, st);
   if (s || !p.parts) return s;
-  if ((int64_t)a.c.max_q * a.H > 0x7fffffff) return EMBER_ERR_SHAPE;
-  const dim3 grid((unsigned)(a.c.max_q * a.H), a.c.n_seqs);
-  if (a.type == EMBER_TYPE_BF16) attn_join_kernel<EMBER_TYPE_BF16><<<grid, 256, 0, st>>>(a, parts);
-  else attn_join_kernel<EMBER_TYPE_F16><<<grid, 256, 0, st>>>(a, parts);
-  return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
+  return a.type == EMBER_TYPE_BF16 ? launch_join<EMBER_TYPE_BF16>(a, parts, st) : launch_join<EMBER_TYPE_F16>(a, parts, st);
 }
 
 }  // namespace ember_attn_impl

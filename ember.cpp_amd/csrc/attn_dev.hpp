@@ -141,16 +141,36 @@ __device__ inline Span visible(const AttnArgs& a, int64_t p, int len, int prefix
   return {lo, (int)min((int64_t)len, max(p + 1, (int64_t)prefix))};
 }
 
-// A score in units of log2: c = scale log2(e), or where it is capped c = scale * 2 / softcap * log2(e) for the exponential in tanh
-// x = 1 - 2 / (1 + exp(2 x)), whose error is absolute, a few 2^-24 of the cap.
+// Scores in units of log2 from products s: c = scale log2(e); where they are capped c = scale * 2 / softcap * log2(e), for the exponential in
+// tanh x = 1 - 2 / (1 + exp(2 x)), whose error is absolute, a few 2^-24 of the cap. Both options are the same for a launch: loops of their own.
 struct Scores {
-  float c, cap, slope;  // cap: softcap * log2(e), 0 if there is none; slope: slopes[h] * log2(e)
-  __device__ float operator()(float s, int dist) const {
-    float t = s * c;
-    if (cap > 0.0f) t = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(t)));
-    return t - slope * (float)abs(dist);
+  float c, cap, slope;  // cap: softcap * log2(e), 0 if there is none; slope: slopes[h] * log2(e), used if `sloped`
+  bool sloped;
+  // N scores, of the keys at distance dist + key(i)
+  template <int N, class S, class K>
+  __device__ __forceinline__ void operator()(S&& s, int dist, K key) const {
+    if (cap > 0.0f) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s(i) = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + exp2_fast(s(i) * c)), cap);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s(i) *= c;
+    }
+    if (sloped) {
+      const float d = (float)dist;
+#pragma unroll
+      for (int i = 0; i < N; ++i) s(i) = __builtin_fmaf(-slope, __builtin_fabsf(d + (float)key(i)), s(i));
+    }
   }
 };
+// -inf for the scores of keys outside [from, to), key(i) being score i's.
+template <int N, class S, class K>
+__device__ __forceinline__ void mask_scores(S&& s, int from, int to, K key) {
+  const uint32_t span = (uint32_t)max(to - from, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if ((uint32_t)(key(i) - from) >= span) s(i) = -INFINITY;
+}
 
 // Where partial results go: for part s and row r of the call (token * n_heads + head) the sum of weighted values o[s][r][D], not
 // yet divided, and the maximum (log2 units) and sum of weights ml[s][r][2].

@@ -256,26 +256,18 @@ __global__ __launch_bounds__(kStepThreads, DP > 128 ? (Op<T>::kQ8 ? 2 : 1) : Op<
 
     uint64_t bad = __ballot(here == ~0u);  // keys in no page: their scores are NaN
     if constexpr (KT < 64) bad &= (1ull << KT) - 1;
-    const Scores sc{c_row, cap, slope};
     float x[NT * 4];
 #pragma unroll
-    for (int i = 0; i < NT * 4; ++i) {  // key of score i: 16 (i / 4) + 4 g + i % 4
-      const int key = (i >> 2) * 16 + g * 4 + (i & 3);
-      x[i] = GEN ? sc(s[i >> 2][i & 3], kt + key - pos) : s[i >> 2][i & 3] * c_row;
-    }
+    for (int i = 0; i < NT * 4; ++i) x[i] = s[i >> 2][i & 3];
+    auto score = [&](int i) -> float& { return x[i]; };
+    auto key_of = [](int i) { return (i >> 2) * 16 + (i & 3); };  // (4 g further)
+    Scores{c_row, cap, slope, GEN && a.slopes}.template operator()<NT * 4>(score, kt + g * 4 - pos, key_of);
     if (bad) {
 #pragma unroll
       for (int i = 0; i < NT * 4; ++i)
-        if (bad >> ((i >> 2) * 16 + g * 4 + (i & 3)) & 1) x[i] = __builtin_nanf("");
+        if (bad >> (key_of(i) + g * 4) & 1) x[i] = __builtin_nanf("");
     }
-    if (masked) {
-      const int from = max(see.lo, lo) - kt - g * 4, to = min(see.hi, hi) - kt - g * 4;
-#pragma unroll
-      for (int i = 0; i < NT * 4; ++i) {
-        const int key = (i >> 2) * 16 + (i & 3);
-        if (key < from || key >= to) x[i] = -INFINITY;
-      }
-    }
+    if (masked) mask_scores<NT * 4>(score, max(see.lo, lo) - kt - g * 4, min(see.hi, hi) - kt - g * 4, key_of);
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < NT * 4; ++i) top = fmaxf(top, x[i]);

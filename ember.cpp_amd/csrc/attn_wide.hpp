@@ -67,12 +67,14 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
   __shared__ unsigned long long odd_keys[4];  // of tile n at n % 4: its keys whose values are not all finite
   const CacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, n32 = lane & 31;
-  // the block: KV head fastest (of 8, each stays on one XCD, whose L2 then holds its keys for all row tiles), the last rows, which
-  // see the most keys, first
+  // the block: KV head fastest (of 8, each stays on one XCD, whose L2 then holds its keys for all row tiles); the last rows, which
+  // see the most keys, first. Where all blocks find a place at once (512), the second half in the other order, so that a CU's two are
+  // a long and a short one
   int x = blockIdx.x;
   const int kvh = x % c.n_kv;
   x /= c.n_kv;
-  const int split = x % splits, r0 = (tiles - 1 - x / splits) * kWideRows;
+  const int split = x % splits, turn = x / splits, half_ = (tiles + 1) / 2;
+  const int r0 = (gridDim.x * gridDim.y <= 512 && turn >= half_ ? turn - half_ : tiles - 1 - turn) * kWideRows;
   const int kv_seq = SHARED ? 0 : blockIdx.y;
   int first = 0, count = c.n_tokens, len = 0, prefix = 0;
   int64_t p0 = 0;
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
       mul = fminf(__builtin_ldexpf(mul, e), 3e38f);
     }
   }
-  const Scores sc{mul, GEN && a.softcap > 0.0f ? a.softcap * kLog2e : 0.0f, GEN && a.slopes && ok ? a.slopes[h] * kLog2e : 0.0f};
+  const Scores sc{mul, GEN && a.softcap > 0.0f ? a.softcap * kLog2e : 0.0f, GEN && a.slopes && ok ? a.slopes[h] * kLog2e : 0.0f, a.slopes != nullptr};
   const int pos = (int)p;
   if (!ok) see = {0, INT32_MAX};
 
@@ -306,20 +308,11 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
       lds_ahead<NS * KS, 1, 6>();
       // key of score i of half-tile u: 8 (i / 4) + 4 half + i % 4
       const bool masked = kt < all_lo || kt + KT > all_hi;
-      if (GEN) {
-#pragma unroll
-        for (int u = 0; u < NS; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[u][i] = sc(s[u][i], kt + u * 32 + 8 * (i >> 2) + 4 * half + (i & 3) - pos);
-      }
+      auto score = [&](int i) -> float& { return reinterpret_cast<float*>(&s[i >> 4])[i & 15]; };
+      auto key_of = [](int i) { return (i >> 4) * 32 + 8 * (i >> 2 & 3) + (i & 3); };
+      if (GEN) sc.template operator()<NS * 16>(score, kt + 4 * half - pos, key_of);
       if (masked) {
-#pragma unroll
-        for (int u = 0; u < NS; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = kt + u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-            if (key < see.lo || key >= see.hi) s[u][i] = -INFINITY;
-          }
+        mask_scores<NS * 16>(score, see.lo - kt - 4 * half, see.hi - kt - 4 * half, key_of);
         if (const uint64_t odd = odd_keys[n & 3]) {  // a row that sees one of them: NaN by its sum of weights
           const int from = max(see.lo - kt, 0), to = min(see.hi - kt, KT);
           if (from < to && (odd >> from & (~0ull >> (64 - (to - from))))) l = __builtin_nanf("");
