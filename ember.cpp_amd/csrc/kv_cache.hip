@@ -12,8 +12,9 @@ namespace ember_attn_impl {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;       // chunks per thread: the look-up is paid once for 1024 of them
-constexpr int kMaxTok = 258;    // tokens that 1024 chunks touch: rows have at least 4 chunks
+// Chunks of K, and as many of V, per thread: their loads are all on the way before the first is used. One where blocks are few: their
+// look-ups are then all of their time.
+constexpr int kManyItems = 4;
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -23,57 +24,88 @@ constexpr int64_t kNoSeq = -1, kNoPage = -2;
 
 // Cache row of token i (cache_row); kNoSeq: the row belongs to no sequence; kNoPage: its place is in no page.
 __device__ inline int64_t token_place(const CacheArgs& c, int i, int lane) {
-  int b = i;
+  int b = i, first = i, end = i + 1, len = 0;
   if (c.q_start) {
-    b = 0;
-    for (int s = 0; s < c.n_seqs; s += 64) {
-      const bool below = s + lane < c.n_seqs && c.q_start[s + lane + 1] <= i;
-      const int n = __popcll(__ballot(below));
-      b += n;
+    // 64 sequences at a time: their starts, ends and lengths at once, then the lane whose sequence it is
+    int s = 0, n = 64;
+    for (; s < c.n_seqs; s += 64) {
+      const bool in = s + lane < c.n_seqs;
+      first = in ? c.q_start[s + lane] : 0;
+      end = in ? c.q_start[s + lane + 1] : INT32_MAX;
+      len = in ? c.kv_len[s + lane] : 0;
+      n = __popcll(__ballot(end <= i));
       if (n < 64) break;
     }
+    b = s + n;
+    if (b >= c.n_seqs) return kNoSeq;
+    first = __builtin_amdgcn_readlane(first, n);
+    end = __builtin_amdgcn_readlane(end, n);
+    len = __builtin_amdgcn_readlane(len, n);
+  } else {
+    if (b >= c.n_seqs) return kNoSeq;
+    len = c.kv_len[b];
   }
-  if (b >= c.n_seqs) return kNoSeq;
-  int first, count;
-  seq_rows(c, b, first, count);
-  // (the sequence's own count, not what n_tokens leaves of it, is what ends at its length)
-  const int len = seq_len(c, b), total = c.q_start ? c.q_start[b + 1] - first : 1;
-  if (i < first || i - first >= count) return kNoSeq;
-  const int64_t pos = (int64_t)len - total + (i - first);
+  if (i < first || first < 0 || i >= c.n_tokens) return kNoSeq;
+  const int64_t pos = (int64_t)max(0, min(len, c.cap)) - ((int64_t)end - first) + (i - first);
   if (pos < 0 || pos >= c.cap) return kNoPage;
   const int64_t row = cache_row(c, b, (int)pos);
   return row < 0 ? kNoPage : row;
 }
 
+// 8 values of type T as they lie in memory: of Q8_0 their codes.
 template <int T>
-__device__ inline void load8(const void* p, int64_t at, float (&x)[8]) {
-  if constexpr (T == EMBER_TYPE_F32) {
-    const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
-    const f32x4 a = s[0], b = s[1];
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-  } else if constexpr (T == EMBER_TYPE_F16) {
-    const h8 a = *reinterpret_cast<const h8*>(static_cast<const _Float16*>(p) + at);
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+struct Raw {
+  uint32_t w[T == EMBER_TYPE_F32 ? 8 : T == EMBER_TYPE_Q8_0 ? 2 : 4];
+};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int T>
+__device__ inline Raw<T> load8(const void* p, int64_t at) {
+  Raw<T> r;
+  if constexpr (T == EMBER_TYPE_Q8_0) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(static_cast<const char*>(p) + at);
+    r.w[0] = a[0], r.w[1] = a[1];
   } else {
-    const u16x8 a = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(p) + at);
-    for (int i = 0; i < 8; ++i) x[i] = ember_moe::bf16_f32(a[i]);
+    const u32x4* s = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (T == EMBER_TYPE_F32 ? 4 : 2));
+    for (int i = 0; i < (T == EMBER_TYPE_F32 ? 2 : 1); ++i) {
+      const u32x4 a = s[i];
+      for (int e = 0; e < 4; ++e) r.w[4 * i + e] = a[e];
+    }
+  }
+  return r;
+}
+template <int T>
+__device__ inline void save8(void* p, int64_t at, const Raw<T>& r) {
+  if constexpr (T == EMBER_TYPE_Q8_0) {
+    *reinterpret_cast<u32x2*>(static_cast<char*>(p) + at) = u32x2{r.w[0], r.w[1]};
+  } else {
+    u32x4* s = reinterpret_cast<u32x4*>(static_cast<char*>(p) + at * (T == EMBER_TYPE_F32 ? 4 : 2));
+    for (int i = 0; i < (T == EMBER_TYPE_F32 ? 2 : 1); ++i) s[i] = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
   }
 }
 template <int T>
-__device__ inline void save8(void* p, int64_t at, const float (&x)[8]) {
-  if constexpr (T == EMBER_TYPE_F32) {
-    f32x4* s = reinterpret_cast<f32x4*>(static_cast<float*>(p) + at);
-    s[0] = f32x4{x[0], x[1], x[2], x[3]};
-    s[1] = f32x4{x[4], x[5], x[6], x[7]};
-  } else if constexpr (T == EMBER_TYPE_F16) {
-    h8 a;
-    for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];
-    *reinterpret_cast<h8*>(static_cast<_Float16*>(p) + at) = a;
-  } else {
-    u16x8 a;
-    for (int i = 0; i < 8; ++i) a[i] = ember_moe::bf16_rne(x[i]);
-    *reinterpret_cast<u16x8*>(static_cast<uint16_t*>(p) + at) = a;
+__device__ inline void values(const Raw<T>& r, float (&x)[8]) {
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (T == EMBER_TYPE_F32) x[i] = __uint_as_float(r.w[i]);
+    else if constexpr (T == EMBER_TYPE_Q8_0) x[i] = (float)(int8_t)(r.w[i / 4] >> (8 * (i % 4)));
+    else if constexpr (T == EMBER_TYPE_BF16) x[i] = ember_moe::bf16_f32((uint16_t)(r.w[i / 2] >> (16 * (i % 2))));
+    else x[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(r.w[i / 2] >> (16 * (i % 2))));
   }
+}
+template <int T>
+__device__ inline Raw<T> raw(const float (&x)[8]) {
+  Raw<T> r;
+  if constexpr (T == EMBER_TYPE_F32) {
+    for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(x[i]);
+  } else {
+    for (int i = 0; i < 4; ++i) {
+      uint32_t h[2];
+      for (int e = 0; e < 2; ++e)
+        h[e] = T == EMBER_TYPE_BF16 ? ember_moe::bf16_rne(x[2 * i + e]) : __builtin_bit_cast(uint16_t, (_Float16)x[2 * i + e]);
+      r.w[i] = h[0] | h[1] << 16;
+    }
+  }
+  return r;
 }
 
 // The code of x at scale d (h = d / 2, inv ~ 1 / d): the integer nearest to the exact quotient, ties to even. n is at
@@ -94,71 +126,90 @@ struct Rows {
   int64_t ks, vs;
 };
 
-template <int T, int C, bool STORE>
-__global__ __launch_bounds__(kThreads) void kv_rows_kernel(CacheArgs c, Rows r, FastDiv chunks) {
-  __shared__ int64_t place[kMaxTok];
-  const int64_t total = (int64_t)c.n_tokens * chunks.d;
-  const int64_t base = (int64_t)blockIdx.x * (kThreads * kItems);
-  const int i0 = (int)(base / chunks.d);
-  const int i1 = (int)((min(base + kThreads * kItems, total) - 1) / chunks.d);
+// Eight values into the cache at `to`, the scale's place being `row`.
+template <int C>
+__device__ inline void put(void* held, _Float16* scales, int64_t to, int64_t scale_at, bool first, float (&x)[8]) {
+  if constexpr (C == EMBER_TYPE_Q8_0) {
+    float m = 0.0f;
+    bool nan = false;
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i])), nan |= x[i] != x[i];
+    if (nan) m = __builtin_nanf("");
+    for (int s = 1; s <= 2; s <<= 1) {
+      const float o = __shfl_xor(m, s, 4);
+      m = m != m || o != o ? __builtin_nanf("") : fmaxf(m, o);
+    }
+    const float q = m / 127.0f;
+    const _Float16 dh = (_Float16)(q > 515.5f ? 515.5f : q);  // (NaN passes)
+    const float d = (float)dh, h = 0.5f * d, inv = 1.0f / d;
+    Raw<C> r = {{0, 0}};
+    if (d > 0.0f)
+      for (int i = 0; i < 8; ++i) r.w[i / 4] |= (uint32_t)(uint8_t)code_of(x[i], d, h, inv) << (8 * (i % 4));
+    save8<C>(held, to, r);
+    if (first) scales[scale_at] = dh;
+  } else {
+    save8<C>(held, to, raw<C>(x));
+  }
+}
+
+template <int T, int C, bool STORE, int kItems>
+__global__ __launch_bounds__(kThreads) void kv_rows_kernel(CacheArgs c, Rows r, FastDiv chunks, FastDiv per_head) {
+  constexpr int kBlock = kThreads * kItems;
+  __shared__ int64_t place[kBlock / 4 + 2];  // of the tokens that the block's chunks touch: rows have at least 4 chunks
+  const int64_t total = (int64_t)c.n_tokens * chunks.d, base = (int64_t)blockIdx.x * kBlock;
+  const int64_t last = min(base + kBlock, total) - 1;
+  const int i0 = base < 0x7fffffff ? (int)div_by((uint32_t)base, chunks) : (int)(base / chunks.d);
+  const int i1 = last < 0x7fffffff ? (int)div_by((uint32_t)last, chunks) : (int)(last / chunks.d);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = i0 + wave; i <= i1; i += kThreads / 64) {
     const int64_t p = token_place(c, i, lane);
     if (lane == 0) place[i - i0] = p;
   }
   __syncthreads();
-  const bool is_v = blockIdx.y != 0;
-  void* rows = is_v ? r.v : r.k;
-  const int64_t stride = is_v ? r.vs : r.ks;
-  void* held = is_v ? c.v : c.k;
-  _Float16* scales = is_v ? c.vs : c.ks;
   const uint32_t off0 = (uint32_t)(base - (int64_t)i0 * chunks.d);  // chunk of token i0 that the block begins with
-  const int per_head = c.D / 8;
+  // Item u's places. (Whole rows and blocks of 32 values: the four lanes of one do the same, or nothing.)
+  int64_t in_k[kItems], in_v[kItems], at[kItems], scale_at[kItems];
+  bool todo[kItems], zero[kItems], first[kItems];
+  constexpr int L = STORE ? T : C;  // what is loaded
+  Raw<L> k[kItems], v[kItems];
+  _Float16 ks[kItems], vs[kItems];
 #pragma unroll
   for (int u = 0; u < kItems; ++u) {
-    const uint32_t n = u * kThreads + threadIdx.x;
-    if (base + n >= total) continue;  // (whole rows, so all four lanes of a block of 32 or none)
-    const uint32_t at = off0 + n, tok = div_by(at, chunks);
+    const uint32_t n = u * kThreads + threadIdx.x, f = off0 + n, tok = min(div_by(f, chunks), (uint32_t)(i1 - i0));
     const int64_t p = place[tok];
-    const int ch = (int)(at - tok * chunks.d), head = ch / per_head, d8 = ch - head * per_head;
-    const int64_t row = p + (int64_t)head * c.page.d;
-    const int64_t in = (int64_t)(i0 + tok) * stride + ch * 8, to = row * c.D + d8 * 8;
-    float x[8];
+    const uint32_t ch = f - tok * chunks.d, head = div_by(ch, per_head), d8 = ch - head * per_head.d;
+    todo[u] = base + n < total && p != kNoSeq && (!STORE || p >= 0);
+    zero[u] = p < 0;
+    const int64_t row = (zero[u] ? 0 : p) + (int64_t)head * c.page.d;
+    in_k[u] = (int64_t)(i0 + tok) * r.ks + ch * 8;
+    in_v[u] = (int64_t)(i0 + tok) * r.vs + ch * 8;
+    at[u] = row * c.D + d8 * 8;
+    scale_at[u] = row * (c.D / 32) + d8 / 4;
+    first[u] = (d8 & 3) == 0;
+    if (todo[u]) {
+      k[u] = load8<L>(STORE ? r.k : c.k, STORE ? in_k[u] : at[u]);
+      v[u] = load8<L>(STORE ? r.v : c.v, STORE ? in_v[u] : at[u]);
+      if constexpr (!STORE && C == EMBER_TYPE_Q8_0) {
+        ks[u] = c.ks[scale_at[u]];
+        vs[u] = c.vs[scale_at[u]];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kItems; ++u) {
+    if (!todo[u]) continue;
+    float x[8], y[8];
+    values<L>(k[u], x);
+    values<L>(v[u], y);
     if constexpr (STORE) {
-      if (p < 0) continue;  // (the same for the four lanes)
-      load8<T>(rows, in, x);
-      if constexpr (C == EMBER_TYPE_Q8_0) {
-        float m = 0.0f;
-        bool nan = false;
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i])), nan |= x[i] != x[i];
-        if (nan) m = __builtin_nanf("");
-        for (int s = 1; s <= 2; s <<= 1) {
-          const float o = __shfl_xor(m, s, 4);
-          m = m != m || o != o ? __builtin_nanf("") : fmaxf(m, o);
-        }
-        const float q = m / 127.0f;
-        const _Float16 dh = (_Float16)(q > 515.5f ? 515.5f : q);  // (NaN passes)
-        const float d = (float)dh, h = 0.5f * d, inv = 1.0f / d;
-        uint64_t codes = 0;
-        if (d > 0.0f)
-          for (int i = 0; i < 8; ++i) codes |= (uint64_t)(uint8_t)code_of(x[i], d, h, inv) << (8 * i);
-        *reinterpret_cast<uint64_t*>(static_cast<int8_t*>(held) + to) = codes;
-        if ((d8 & 3) == 0) scales[row * (c.D / 32) + d8 / 4] = dh;
-      } else {
-        save8<C>(held, to, x);
-      }
+      put<C>(c.k, c.ks, at[u], scale_at[u], first[u], x);
+      put<C>(c.v, c.vs, at[u], scale_at[u], first[u], y);
     } else {
-      if (p < 0) {
-        if (p == kNoSeq) continue;
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      } else if constexpr (C == EMBER_TYPE_Q8_0) {
-        const uint64_t codes = *reinterpret_cast<const uint64_t*>(static_cast<const int8_t*>(held) + to);
-        const float d = (float)scales[row * (c.D / 32) + d8 / 4];
-        for (int i = 0; i < 8; ++i) x[i] = d * (float)(int8_t)(codes >> (8 * i));
-      } else {
-        load8<C>(held, to, x);
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (C == EMBER_TYPE_Q8_0) x[i] *= (float)ks[u], y[i] *= (float)vs[u];
+        if (zero[u]) x[i] = y[i] = 0.0f;
       }
-      save8<T>(rows, in, x);
+      save8<T>(r.k, in_k[u], raw<T>(x));
+      save8<T>(r.v, in_v[u], raw<T>(y));
     }
   }
 }
@@ -166,14 +217,17 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(CacheArgs c, Rows r, 
 template <int T, bool STORE>
 int launch(const CacheArgs& c, const Rows& r, hipStream_t st) {
   const uint32_t per_row = (uint32_t)(c.n_kv * c.D / 8);
-  const int64_t blocks = ((int64_t)c.n_tokens * per_row + kThreads * kItems - 1) / (kThreads * kItems);
+  const int64_t chunks = (int64_t)c.n_tokens * per_row;
+  const bool many = chunks >= (int64_t)512 * kThreads * kManyItems;
+  const int64_t block = kThreads * (many ? kManyItems : 1), blocks = (chunks + block - 1) / block;
   if (blocks > 0x7fffffff) return EMBER_ERR_SHAPE;
-  const dim3 grid((unsigned)blocks, 2);
-  const FastDiv f = fast_div(per_row);
+  const FastDiv f = fast_div(per_row), h = fast_div((uint32_t)c.D / 8);
+  auto go = [&](auto* kernel) { kernel<<<(unsigned)blocks, kThreads, 0, st>>>(c, r, f, h); };
+  auto pick = [&](auto* few, auto* lots) { many ? go(lots) : go(few); };
   switch (c.type) {
-    case EMBER_TYPE_F16: kv_rows_kernel<T, EMBER_TYPE_F16, STORE><<<grid, kThreads, 0, st>>>(c, r, f); break;
-    case EMBER_TYPE_BF16: kv_rows_kernel<T, EMBER_TYPE_BF16, STORE><<<grid, kThreads, 0, st>>>(c, r, f); break;
-    default: kv_rows_kernel<T, EMBER_TYPE_Q8_0, STORE><<<grid, kThreads, 0, st>>>(c, r, f); break;
+    case EMBER_TYPE_F16: pick(kv_rows_kernel<T, EMBER_TYPE_F16, STORE, 1>, kv_rows_kernel<T, EMBER_TYPE_F16, STORE, kManyItems>); break;
+    case EMBER_TYPE_BF16: pick(kv_rows_kernel<T, EMBER_TYPE_BF16, STORE, 1>, kv_rows_kernel<T, EMBER_TYPE_BF16, STORE, kManyItems>); break;
+    default: pick(kv_rows_kernel<T, EMBER_TYPE_Q8_0, STORE, 1>, kv_rows_kernel<T, EMBER_TYPE_Q8_0, STORE, kManyItems>); break;
   }
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }
