@@ -247,7 +247,7 @@ def dequantize(type_id: int, raw: np.ndarray, n: int) -> np.ndarray:
 # Device entry points (torch tensors on the GPU; stream defaults to torch's current stream)
 
 
-def _stream(stream) -> int:
+def _stream(stream, device: Optional[int] = None) -> int:
     if stream is not None:
         return int(stream)
     import torch
@@ -255,7 +255,7 @@ def _stream(stream) -> int:
     # (torch.cuda.current_stream() builds a stream object, 3 us; this is what it asks)
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is not None:
-        return int(raw(torch.cuda.current_device()))
+        return int(raw(torch.cuda.current_device() if device is None else device))
     return int(torch.cuda.current_stream().cuda_stream)
 
 

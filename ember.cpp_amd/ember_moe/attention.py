@@ -61,14 +61,15 @@ def type_id(t) -> int:
     return ty
 
 
-def on_current_device(*tensors) -> None:
-    """Refuses tensors that are not on the current device: the library launches there."""
+def on_current_device(*tensors) -> int:
+    """Refuses tensors that are not on the current device, where the library launches; its index."""
     import torch
 
     here = torch.cuda.current_device()
     for t in tensors:
         if t.get_device() != here:  # (-1 for a CPU tensor)
             raise em.EmberError(em.ERR_LAUNCH, f"tensor on {t.device}, the current device is cuda:{here}")
+    return here
 
 
 def _array(t, n: int, dtype, what: str) -> int:
@@ -169,12 +170,14 @@ class DeviceKvCache:
         return DeviceKvCache(type_, k, v, *(torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.float16, device=device) for _ in range(2)))
 
     def _kv(self, fn: str, batch: KvBatch, k, v, stream):
-        d = self.desc
-        ks, vs = (_rows(t, batch.n_tokens, d.n_kv, d.head_dim, n) for t, n in ((k, "k"), (v, "v")))
+        d, n = self.desc, batch.n_tokens
+        heads, dim = d.n_kv, d.head_dim
+        ks, vs = _rows(k, n, heads, dim, "k"), _rows(v, n, heads, dim, "v")
+        ty = type_id(k)
         if k.dtype != v.dtype:
             raise em.EmberError(em.ERR_TYPE, "k and v of one type are needed")
-        on_current_device(k, v)
-        st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, type_id(k), em._stream(stream))
+        here = on_current_device(k, v)
+        st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, ty, em._stream(stream, here))
         if st:
             raise em.EmberError(st, fn)
         return k, v
@@ -206,9 +209,9 @@ class DeviceKvCache:
             raise em.EmberError(em.ERR_SHAPE, "prefix: one length per sequence is needed")
         if scratch is None:
             scratch = torch.empty(max(1, self.attn_scratch_bytes(opts, batch)), dtype=torch.uint8, device=q.device)
-        on_current_device(q, out, scratch)
+        here = on_current_device(q, out, scratch)
         st = em.lib().ember_attn(ctypes.byref(opts), ctypes.byref(d), ctypes.byref(batch), q.data_ptr(), qs, out.data_ptr(), os_,
-                                 type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream))
+                                 type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream, here))
         if st:
             raise em.EmberError(st, "ember_attn")
         return out

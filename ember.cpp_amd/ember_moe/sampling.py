@@ -59,8 +59,8 @@ def sample(sampler: Sampler, logits, u, ids=None, probs=None, stream=None):
         probs = torch.empty(n, dtype=torch.float32, device=logits.device)
     stride = logits.stride(0) if n > 1 else max(logits.stride(0), V)
     a = (_array(u, n, torch.float32, "u"), _array(ids, n, torch.int32, "ids"), _array(probs, n, torch.float32, "probs"))
-    on_current_device(logits, u, ids, probs)
-    st = em.lib().ember_sample(ctypes.byref(sampler), logits.data_ptr(), type_id(logits), n, V, stride, *a, em._stream(stream))
+    here = on_current_device(logits, u, ids, probs)
+    st = em.lib().ember_sample(ctypes.byref(sampler), logits.data_ptr(), type_id(logits), n, V, stride, *a, em._stream(stream, here))
     if st:
         raise em.EmberError(st, "ember_sample")
     return ids, probs
