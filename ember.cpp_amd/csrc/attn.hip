@@ -90,13 +90,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, Parts parts)
   *reinterpret_cast<u2*>(static_cast<uint16_t*>(a.out) + (int64_t)(first + tok) * a.out_stride + (int64_t)h * c.D + d) = y;
 }
 
+int64_t join_blocks(const AttnArgs& a, int parts) {
+  const int64_t rows = (int64_t)a.c.max_q * a.H;
+  return parts <= kFewParts ? (rows + 3) / 4 : rows;
+}
 template <int IO>
 int launch_join(const AttnArgs& a, const Parts& parts, hipStream_t st) {
-  const int64_t rows = (int64_t)a.c.max_q * a.H;
-  const bool few = parts.n <= kFewParts;
-  if (rows > 0x7fffffff) return EMBER_ERR_SHAPE;
-  const dim3 grid((unsigned)(few ? (rows + 3) / 4 : rows), a.c.n_seqs);
-  if (few) attn_join_kernel<IO, 1><<<grid, 256, 0, st>>>(a, parts);
+  const dim3 grid((unsigned)join_blocks(a, parts.n), a.c.n_seqs);
+  if (parts.n <= kFewParts) attn_join_kernel<IO, 1><<<grid, 256, 0, st>>>(a, parts);
   else attn_join_kernel<IO, 4><<<grid, 256, 0, st>>>(a, parts);
   return hipGetLastError() == hipSuccess ? EMBER_OK : EMBER_ERR_LAUNCH;
 }
@@ -147,6 +148,10 @@ size_t attn_scratch(const AttnArgs& a) {
 
 int launch_attn(const AttnArgs& a, void* scratch, hipStream_t st) {
   const AttnPlan p = attn_plan(a);
+  auto tiles = [&](int64_t tokens) { return (tokens * a.G + 127) / 128 * a.c.n_kv; };  // of attn_wide_kernel
+  if ((p.begin && tiles(a.c.n_tokens) * p.shared_splits > kMaxBlocks) || (!p.step && tiles(a.c.max_q) * p.splits > kMaxBlocks) ||
+      (p.parts && join_blocks(a, p.parts) > kMaxBlocks))
+    return EMBER_ERR_SHAPE;
   Parts parts{nullptr, nullptr, (int64_t)a.c.n_tokens * a.H, std::max(p.parts, 1)};
   if (p.parts) {
     parts.o = static_cast<float*>(scratch);

@@ -17,8 +17,8 @@ inline FastDiv fast_div(uint32_t d) {
   while ((1ull << s) < d) ++s;
   return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
 }
-__device__ inline uint32_t div_by(uint32_t n, const FastDiv& f) {
-  return (__umulhi(n, f.mul) + n) >> f.shift;
+__host__ __device__ inline uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return ((uint32_t)((uint64_t)n * f.mul >> 32) + n) >> f.shift;
 }
 
 // A call's cache and batch as the kernels take them.
@@ -36,27 +36,44 @@ struct CacheArgs {
   const int32_t* pages;    // or null
 };
 
+// Where the device arrays point, kept inside the buffers whatever they hold (host code too, for its test on the CPU).
+
 // Index of the cache row (page, KV head 0, row in the page) in units of [page] rows of one head: the page's first row
 // is pid * n_kv * page. -1: no such page.
-__device__ inline int64_t cache_row(const CacheArgs& c, int b, int pos) {
+__host__ __device__ inline int64_t cache_row(const CacheArgs& c, int b, int pos) {
   const uint32_t pg = div_by((uint32_t)pos, c.page);
   const int pid = c.pages ? c.pages[(int64_t)b * c.max_pages + pg] : b;
   if ((uint32_t)pid >= (uint32_t)c.n_pages) return -1;
   return (int64_t)pid * c.n_kv * c.page.d + (pos - (int)(pg * c.page.d));
 }
-__device__ inline int seq_len(const CacheArgs& c, int b) { return max(0, min(c.kv_len[b], c.cap)); }
+__host__ __device__ inline int length(const CacheArgs& c, int len) { return len < 0 ? 0 : len < c.cap ? len : c.cap; }
+__device__ inline int seq_len(const CacheArgs& c, int b) { return length(c, c.kv_len[b]); }
+
+constexpr int64_t kNoSeq = -1, kNoPage = -2;
+// Cache row of token i, which is of sequence b, whose rows are first .. end - 1 and whose length is len;
+// kNoSeq: the row belongs to no sequence; kNoPage: its place is in no page.
+__host__ __device__ inline int64_t place_of(const CacheArgs& c, int b, int first, int end, int len, int i) {
+  if (b >= c.n_seqs || i < first || first < 0 || i >= c.n_tokens) return kNoSeq;
+  const int64_t pos = (int64_t)length(c, len) - ((int64_t)end - first) + (i - first);
+  if (pos < 0 || pos >= c.cap) return kNoPage;
+  const int64_t row = cache_row(c, b, (int)pos);
+  return row < 0 ? kNoPage : row;
+}
 
 // Rows of sequence b: first row and count, kept inside [0, n_tokens).
-__device__ inline void seq_rows(const CacheArgs& c, int b, int& first, int& count) {
+__host__ __device__ inline void seq_rows(const CacheArgs& c, int b, int& first, int& count) {
   if (!c.q_start) {
     first = b;
     count = 1;
     return;
   }
   first = c.q_start[b];
-  const int end = min(c.q_start[b + 1], c.n_tokens);
-  count = first < 0 ? 0 : max(0, end - first);
+  const int last = c.q_start[b + 1], end = last < c.n_tokens ? last : c.n_tokens;
+  count = first < 0 || end < first ? 0 : end - first;
 }
+
+// Blocks of 256 threads that a launch can have in x: the runtime counts threads in 32 bits.
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;
 
 int make_cache_args(const ember_kv_cache* c, const ember_kv_batch* b, CacheArgs* out);
 

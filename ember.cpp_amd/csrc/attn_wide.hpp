@@ -393,7 +393,6 @@ __global__ __launch_bounds__(kWideThreads, DP <= 128 ? 2 : 1) void attn_wide_ker
 template <int T, int IO, int DP, bool SHARED>
 int launch_wide(const AttnArgs& a, const Parts& p, const WideCall& w, hipStream_t st) {
   const int64_t rows = (int64_t)(SHARED ? a.c.n_tokens : a.c.max_q) * a.G, tiles = (rows + kWideRows - 1) / kWideRows;
-  if (tiles * w.splits * a.c.n_kv > 0x7fffffff) return EMBER_ERR_SHAPE;
   const dim3 grid((unsigned)(tiles * w.splits * a.c.n_kv), SHARED ? 1 : a.c.n_seqs);
   constexpr size_t lds = WideLds<DP>::kBytes;
   static_assert(lds <= 65536, "no attribute needed");

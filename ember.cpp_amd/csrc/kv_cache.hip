@@ -20,9 +20,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int64_t kNoSeq = -1, kNoPage = -2;
-
-// Cache row of token i (cache_row); kNoSeq: the row belongs to no sequence; kNoPage: its place is in no page.
+// Cache row of token i, or what place_of gives in its stead.
 __device__ inline int64_t token_place(const CacheArgs& c, int i, int lane) {
   int b = i, first = i, end = i + 1, len = 0;
   if (c.q_start) {
@@ -45,11 +43,7 @@ __device__ inline int64_t token_place(const CacheArgs& c, int i, int lane) {
     if (b >= c.n_seqs) return kNoSeq;
     len = c.kv_len[b];
   }
-  if (i < first || first < 0 || i >= c.n_tokens) return kNoSeq;
-  const int64_t pos = (int64_t)max(0, min(len, c.cap)) - ((int64_t)end - first) + (i - first);
-  if (pos < 0 || pos >= c.cap) return kNoPage;
-  const int64_t row = cache_row(c, b, (int)pos);
-  return row < 0 ? kNoPage : row;
+  return place_of(c, b, first, end, len, i);
 }
 
 // 8 values of type T as they lie in memory: of Q8_0 their codes.
@@ -220,7 +214,7 @@ int launch(const CacheArgs& c, const Rows& r, hipStream_t st) {
   const int64_t chunks = (int64_t)c.n_tokens * per_row;
   const bool many = chunks >= (int64_t)512 * kThreads * kManyItems;
   const int64_t block = kThreads * (many ? kManyItems : 1), blocks = (chunks + block - 1) / block;
-  if (blocks > 0x7fffffff) return EMBER_ERR_SHAPE;
+  if (blocks > kMaxBlocks) return EMBER_ERR_SHAPE;
   const FastDiv f = fast_div(per_row), h = fast_div((uint32_t)c.D / 8);
   auto go = [&](auto* kernel) { kernel<<<(unsigned)blocks, kThreads, 0, st>>>(c, r, f, h); };
   auto pick = [&](auto* few, auto* lots) { many ? go(lots) : go(few); };

@@ -700,7 +700,8 @@ extern "C" int ember_sample(const ember_sampler* s, const void* logits, int type
                             int32_t* ids, float* probs, hipStream_t stream) {
   if (!s) return EMBER_ERR_NULL;
   if (type != EMBER_TYPE_F32 && type != EMBER_TYPE_F16 && type != EMBER_TYPE_BF16) return EMBER_ERR_TYPE;
-  if (n < 0 || V < 1 || V > (1 << 24) || stride < V || stride > (int64_t)1 << 40) return EMBER_ERR_SHAPE;
+  // (the runtime counts a launch's threads in 32 bits)
+  if (n < 0 || n > (1 << 23) - 1 || V < 1 || V > (1 << 24) || stride < V || stride > (int64_t)1 << 40) return EMBER_ERR_SHAPE;
   if (n == 0) return EMBER_OK;
   if (!logits || !u || !ids) return EMBER_ERR_NULL;
   const uintptr_t size = type == EMBER_TYPE_F32 ? 4 : 2;

@@ -72,6 +72,13 @@ def on_current_device(*tensors) -> int:
     return here
 
 
+def own_stream(stream, here: int, what: str) -> None:
+    """Refuses a stream other than torch's current one for a call that would allocate `what`: the memory is the current stream's, and
+    may be in use there, before the call and after it."""
+    if stream is not None and int(stream) != em._stream(None, here):
+        raise em.EmberError(em.ERR_NULL, f"{what}: needed on a stream other than the current one")
+
+
 def _array(t, n: int, dtype, what: str) -> int:
     """The address of a caller's device array of n values, or 0 for None."""
     if t is None:
@@ -96,7 +103,7 @@ def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: int = 
             raise em.EmberError(em.ERR_SHAPE, "pages: [n_seqs, max_pages] is needed")
         b.pages, b.max_pages = _array(pages, pages.numel(), torch.int32, "pages"), pages.shape[1]
     on_current_device(*(t for t in (kv_len, q_start, pages) if t is not None))
-    b._owner = (kv_len, q_start, pages)
+    b._owner = (kv_len, q_start, pages)  # (all on one device: calls look at the first's)
     return b
 
 
@@ -176,7 +183,7 @@ class DeviceKvCache:
         ty = type_id(k)
         if k.dtype != v.dtype:
             raise em.EmberError(em.ERR_TYPE, "k and v of one type are needed")
-        here = on_current_device(k, v)
+        here = on_current_device(k, v, self.k, *getattr(batch, "_owner", ())[:1])
         st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, ty, em._stream(stream, here))
         if st:
             raise em.EmberError(st, fn)
@@ -199,17 +206,24 @@ class DeviceKvCache:
 
         d = self.desc
         qs = _rows(q, batch.n_tokens, opts.n_heads, d.head_dim, "q")
+        here = on_current_device(q, self.k, *getattr(batch, "_owner", ())[:1])
         if out is None:
+            own_stream(stream, here, "out")
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         os_ = _rows(out, batch.n_tokens, opts.n_heads, d.head_dim, "out")
         if out.dtype != q.dtype:
             raise em.EmberError(em.ERR_TYPE, "q and out of one type are needed")
-        prefix = getattr(opts, "_owner", (None, None))[1]
+        slopes, prefix = getattr(opts, "_owner", (None, None))
         if prefix is not None and prefix.numel() < batch.n_seqs:
             raise em.EmberError(em.ERR_SHAPE, "prefix: one length per sequence is needed")
         if scratch is None:
-            scratch = torch.empty(max(1, self.attn_scratch_bytes(opts, batch)), dtype=torch.uint8, device=q.device)
-        here = on_current_device(q, out, scratch)
+            need = self.attn_scratch_bytes(opts, batch)
+            if need:
+                own_stream(stream, here, "scratch")
+            scratch = torch.empty(max(1, need), dtype=torch.uint8, device=q.device)
+        elif not scratch.is_contiguous():
+            raise em.EmberError(em.ERR_SCRATCH, "scratch: contiguous memory is needed")
+        on_current_device(out, scratch, *(t for t in (slopes, prefix) if t is not None))
         st = em.lib().ember_attn(ctypes.byref(opts), ctypes.byref(d), ctypes.byref(batch), q.data_ptr(), qs, out.data_ptr(), os_,
                                  type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream, here))
         if st:

@@ -5,7 +5,7 @@ import ctypes
 
 import ember_moe as em
 
-from .attention import _array, on_current_device, type_id
+from .attention import _array, on_current_device, own_stream, type_id
 
 
 class Sampler(ctypes.Structure):
@@ -53,13 +53,16 @@ def sample(sampler: Sampler, logits, u, ids=None, probs=None, stream=None):
     n, V = logits.shape
     if getattr(sampler, "_rows", None) is not None and sampler._rows < n:
         raise em.EmberError(em.ERR_SHAPE, f"settings of {sampler._rows} rows for {n}")
+    here = on_current_device(logits, u, *getattr(sampler, "_owner", ()))
+    if ids is None or probs is None:
+        own_stream(stream, here, "ids and probs")
     if ids is None:
         ids = torch.empty(n, dtype=torch.int32, device=logits.device)
     if probs is None:
         probs = torch.empty(n, dtype=torch.float32, device=logits.device)
     stride = logits.stride(0) if n > 1 else max(logits.stride(0), V)
     a = (_array(u, n, torch.float32, "u"), _array(ids, n, torch.int32, "ids"), _array(probs, n, torch.float32, "probs"))
-    here = on_current_device(logits, u, ids, probs)
+    on_current_device(ids, probs)
     st = em.lib().ember_sample(ctypes.byref(sampler), logits.data_ptr(), type_id(logits), n, V, stride, *a, em._stream(stream, here))
     if st:
         raise em.EmberError(st, "ember_sample")

@@ -1,6 +1,8 @@
 """CPU checks of the cache, attention and sampling entries of the C ABI: every declared function is exported, and calls that
 are refused return the documented status before any GPU work."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -118,3 +120,23 @@ def test_sampling_is_checked():
                        (dict(temperatures=0x400002), em.ERR_ALIGN), (dict(top_ks=0x400001), em.ERR_ALIGN)]:
         assert call(**kw) == status, kw
     assert call(n=0, z=0, u=0, ids=0) == em.OK
+
+
+def test_calls_too_large_for_a_launch():
+    """More blocks than a launch can have: refused before anything runs."""
+    big = batch(n_tokens=2**31 - 1, max_q=2**31 - 1, q_start=0x70000, max_kv=112)
+    wide = cache(n_kv=256, head_dim=256, n_pages=16)
+    for fn in ("ember_kv_store", "ember_kv_load"):
+        assert _store(fn, wide, big, ks=65536, vs=65536) == em.ERR_SHAPE
+    assert _attn(opts(n_heads=256), cache(), big, qs=256 * 64, os_=256 * 64) == em.ERR_SHAPE
+    a = em.Sampler()
+    assert em.lib().ember_sample(ctypes.byref(a), 0x100000, em.F32, 1 << 23, 100, 100, 0x200000, 0x300000, 0, None) == em.ERR_SHAPE
+
+
+def test_places_and_plans():
+    """The native check of what keeps the kernels inside their buffers: places of tokens for device arrays of any content, and the
+    parts that a call is split into."""
+    exe = os.path.join(os.path.dirname(__file__), "native", "attn_host_check")
+    assert os.path.exists(exe), f"{exe} is missing: run `make` in ember.cpp_amd/"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout + r.stderr

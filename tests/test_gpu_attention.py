@@ -329,3 +329,43 @@ def test_binding_refuses(gpu):
         s.cache.attend(em.attn_options(4, 64, prefix=torch.zeros(0, dtype=torch.int32, device="cuda")), s.batch, q)
     with pytest.raises(em.EmberError):
         em.attn_options(4, 64, slopes=torch.zeros(3, device="cuda"))
+
+
+def test_binding_refuses_what_another_stream_may_not_have(gpu):
+    """Memory that the binding allocates is the current stream's: a call on another one brings its own."""
+    s = Setup(em.BF16, [(5000, 1)], 2, 128, 64).up()
+    a, q, side = em.attn_options(8, 128), rows(s, 8, torch.bfloat16).cuda(), torch.cuda.Stream()
+    out, scratch = torch.empty_like(q), torch.empty(max(1, s.cache.attn_scratch_bytes(a, s.batch)), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for kw in (dict(), dict(out=out), dict(scratch=scratch)):
+        with pytest.raises(em.EmberError) as e:
+            s.cache.attend(a, s.batch, q, stream=side.cuda_stream, **kw)
+        assert e.value.status == em.ERR_NULL
+    with pytest.raises(em.EmberError):
+        s.cache.attend(a, s.batch, q, out, scratch[:1].expand(scratch.numel()))
+    with pytest.raises(em.EmberError):
+        em.sample(em.Sampler(), torch.zeros(1, 10, device="cuda"), torch.zeros(1, device="cuda"), stream=side.cuda_stream)
+    s.cache.attend(a, s.batch, q, out, scratch, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out, s.cache.attend(a, s.batch, q, stream=torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.parametrize("type_,io", TYPES[1:])
+@pytest.mark.parametrize("page", [4096, 4000])
+def test_far_pages(gpu, type_, io, page):
+    """Pages past 2^32 values (of Q8_0: bytes) of the cache give what the same rows give at its start."""
+    n_kv, D, n_pages = 2, 256, (1 << 32) // (2 * 256 * page) + 4
+    cache = em.DeviceKvCache.create(type_, n_pages, n_kv, page, D)
+    assert cache.k.numel() > 1 << 32
+    near, far = torch.tensor([[1, 0]], dtype=torch.int32).cuda(), torch.tensor([[n_pages - 1, n_pages - 3]], dtype=torch.int32).cuda()
+    kv = torch.tensor([page + 100], dtype=torch.int32).cuda()
+    x, y = (torch.randn(page + 100, n_kv, D, generator=torch.Generator().manual_seed(i)).to(TORCH[io]).cuda() for i in range(2))
+    starts = torch.tensor([0, page + 100], dtype=torch.int32).cuda()
+    for table in (near, far):
+        cache.store(em.kv_batch(kv, starts, n_tokens=page + 100, max_q=page + 100, max_kv=2 * page, pages=table), x, y)
+    a = em.attn_options(8, D)
+    for q_len in (1, 200):
+        q = torch.randn(q_len, 8, D, generator=torch.Generator().manual_seed(q_len)).to(TORCH[io]).cuda()
+        at = torch.tensor([0, q_len], dtype=torch.int32).cuda()
+        got = [cache.attend(a, em.kv_batch(kv, at, n_tokens=q_len, max_q=q_len, max_kv=2 * page, pages=t), q) for t in (near, far)]
+        assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1]) and got[0].float().abs().max() > 0.01
