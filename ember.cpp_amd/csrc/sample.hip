@@ -32,6 +32,7 @@ constexpr int kPer = 16, kCap = kPer * kThreads;  // gathered tokens, kPer * 64 
 constexpr int kCell = 256;                       // tokens that a wave takes at once: 4 a lane, side by side
 constexpr int kAhead = 16;                       // cells per wave whose loads are on the way at once: 128 KB per block
 constexpr int kBinPer = kBins / kThreads;
+static_assert(kBinPer == 4, "find_bin");
 constexpr int kGroupMaxK = 1600;                 // top-k that the maxima of 2048 groups bound well
 typedef unsigned long long u64;
 
@@ -56,11 +57,9 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 struct Shared {
-  u64 bin[kBins];
+  alignas(16) u64 bin[kBins];
   union {
-    struct {
-      uint32_t key[kCap], idx[kCap];
-    };
+    u64 list[kCap];  // gathered: bits of the logit, index above them
     struct {
       u64 cell[kBins];
       uint32_t cell_ties[kBins];
@@ -172,14 +171,19 @@ __device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
 // before it, the sum with it}. Leaves the bins cleared.
 __device__ __forceinline__ void find_bin(Shared& sh, u64* bins, int n, bool down, u64 run, u64 need) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // four bins side by side per thread: 32 bytes at once (downwards n is a multiple of four)
+  typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+  const int at = kBinPer * (int)threadIdx.x, b0 = down ? max(n - kBinPer - at, 0) : at;
+  u64x2* const q = reinterpret_cast<u64x2*>(bins + b0);
+  const u64x2 q0 = q[0], q1 = q[1];
+  if (at < n) q[0] = q[1] = u64x2{0, 0};
+  const u64 y[kBinPer] = {q0[0], q0[1], q1[0], q1[1]};
   u64 x[kBinPer], mine = 0;
   int b[kBinPer];
 #pragma unroll
   for (int e = 0; e < kBinPer; ++e) {
-    const int at = kBinPer * (int)threadIdx.x + e;
-    b[e] = down ? n - 1 - at : at;
-    x[e] = at < n ? bins[b[e]] : 0;
-    if (at < n) bins[b[e]] = 0;
+    b[e] = down ? n - 1 - at - e : at + e;
+    x[e] = at + e >= n ? 0 : down ? y[kBinPer - 1 - e] : y[e];
     mine += x[e];
   }
   const u64 upto = wave_upto(mine);
@@ -201,14 +205,14 @@ __device__ __forceinline__ void find_bin(Shared& sh, u64* bins, int n, bool down
 }
 
 // exp((z - top) / temperature), as p 2^n: 2^f for the fraction f, by its Taylor series to the 11th power (at |f| <= 1/2 the rest is under 2^-47),
-// some 20 instructions. Infinite logits count as 2^200, which is as far from every finite one as it takes.
+// n rounded off by adding 1.5 2^52 and scaled by adding to the exponent: some 25 instructions, no conversion among them but the logit's. Infinite logits count as 2^200, which is as far from every finite one as it takes.
 struct Weigh {
   float top;
   double far, c;  // min(top, 2^200); log2(e) / temperature
   int s;          // weights are summed as integers, times 2^s
   __device__ __forceinline__ double part(float z, int& n) const {
-    const double y = (fmin((double)z, 0x1p200) - far) * c, r = rint(y), f = y - r;
-    n = (int)fmax(r, -100000.0);
+    const double y = fmax((fmin((double)z, 0x1p200) - far) * c, -900.0), t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+    n = (int)(uint32_t)__double_as_longlong(t);
     double p = 4.44553827187081e-10;
     p = __builtin_fma(p, f, 7.054911620801121e-09);
     p = __builtin_fma(p, f, 1.0178086009239696e-07);
@@ -222,17 +226,29 @@ struct Weigh {
     p = __builtin_fma(p, f, 0.6931471805599453);
     return __builtin_fma(p, f, 1.0);
   }
-  __device__ __forceinline__ double e(uint32_t key) const {
+  __device__ __forceinline__ double e(float z) const {
     int n;
-    const double p = part(value_of(key), n);
-    return ldexp(p, n);
+    const double p = part(z, n);
+    return scaled(p, n);
   }
-  // e 2^s to the nearest integer: the low bits of 2^52 plus it
-  __device__ __forceinline__ u64 fix(double e) const { return __double_as_longlong(ldexp(e, s) + 0x1p52) - __double_as_longlong(0x1p52); }
+  __device__ __forceinline__ double e(uint32_t key) const { return e(value_of(key)); }
+  // x 2^n, both normal
+  static __device__ __forceinline__ double scaled(double x, int n) {
+    const u64 b = (u64)__double_as_longlong(x);
+    return __longlong_as_double((long long)((u64)((uint32_t)(b >> 32) + ((uint32_t)n << 20)) << 32 | (uint32_t)b));
+  }
+  // e 2^s (at most 2^51) to the nearest integer: the low bits of 2^52 plus it
+  static __device__ __forceinline__ u64 integer(double e) { return (u64)__double_as_longlong(e + 0x1p52) & 0xfffffffffffffull; }
+  __device__ __forceinline__ u64 fix(double e) const { return integer(scaled(e, s)); }
   __device__ __forceinline__ u64 at(float z) const {
     int n;
     const double p = part(z, n);
-    return __double_as_longlong(ldexp(p, n + s) + 0x1p52) - __double_as_longlong(0x1p52);
+    return integer(scaled(p, n + s));
+  }
+  // Of four, 0 for what is never drawn: side by side, without branches (each step waits for the one before: a token at a time a pass over 131072 took 11 us more).
+  __device__ __forceinline__ void at4(const float (&z)[4], u64 (&x)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = at(fmaxf(z[e], -INFINITY));  // (NaN: -inf, whose weight is 0)
   }
 };
 
@@ -270,8 +286,7 @@ __device__ __forceinline__ bool gather(const R& r, Shared& sh, F is) {
       if (!mask) continue;
       const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
       if (in && at < kPer * 64) {
-        sh.key[base + at] = key_of(z[e]);
-        sh.idx[base + at] = (uint32_t)(i + e);
+        sh.list[base + at] = (u64)(uint32_t)(i + e) << 32 | __float_as_uint(z[e]);
       }
       count += (uint32_t)__popcll(mask);
     }
@@ -288,8 +303,9 @@ __device__ __forceinline__ bool gather(const R& r, Shared& sh, F is) {
 __device__ __forceinline__ bool item(const Shared& sh, int i, uint32_t& key, uint32_t& idx) {
   const int wave = threadIdx.x >> 6, at = i * 64 + (int)(threadIdx.x & 63);
   if (at >= (int)sh.counts[wave]) return false;
-  key = sh.key[wave * kPer * 64 + at];
-  idx = sh.idx[wave * kPer * 64 + at];
+  const u64 x = sh.list[wave * kPer * 64 + at];
+  key = key_of(__uint_as_float((uint32_t)x));
+  idx = (uint32_t)(x >> 32);
   return true;
 }
 __device__ __forceinline__ int items(const Shared& sh) {
@@ -339,12 +355,13 @@ __device__ __forceinline__ void bins_row(const R& r, Shared& sh, const Weigh& w,
   u64 sum = threadIdx.x == 0 ? extra : 0;
   const float above = floor_key ? value_of(floor_key) : -INFINITY;
   r.each([&](int, const float (&z)[4]) {
+    u64 x[4] = {1, 1, 1, 1};
+    if (MASS) w.at4(z, x);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (z[e] > above) {
-        const u64 x = MASS ? w.at(z[e]) : 1ull;
-        if (x) atomicAdd(&sh.bin[bin_of(z[e])], x);
-        sum += x;
+      if (z[e] > above && x[e]) {
+        atomicAdd(&sh.bin[bin_of(z[e])], x[e]);
+        sum += x[e];
       }
   });
   if (extra && threadIdx.x == 0) atomicAdd(&sh.bin[bin_of(above)], extra);
@@ -598,8 +615,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
 
   // Too many to gather: the weights of the tokens above t, and the tokens equal to it, by cells of consecutive tokens, a wave a cell.
   auto weight = [&](float z) -> u64 {
-    const double e = w.e(key_of(z));
-    return e >= (double)min_p ? w.fix(e) : 0;
+    const double e = w.e(fmaxf(z, -INFINITY));
+    return e >= (double)min_p ? Weigh::integer(Weigh::scaled(e, w.s)) : 0;
   };
   const float tz = t ? value_of(t) : -INFINITY;
   const u64 wt = t ? weight(tz) : 0;
@@ -609,10 +626,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Args a) {
     uint32_t eq = 0;
     for (int sub = 0; sub < 1 << a.cell_shift; ++sub) {
       float z[4];
+      u64 y[4];
       r.load(((c << a.cell_shift) + sub) * kCell + lane * 4, z);
 #pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = weight(z[e]);
+#pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (z[e] > tz) x += weight(z[e]);
+        x += z[e] > tz ? y[e] : 0;
         eq += t && z[e] == tz;
       }
     }

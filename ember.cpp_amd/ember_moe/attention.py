@@ -25,6 +25,7 @@ class KvCache(ctypes.Structure):
 class KvBatch(ctypes.Structure):
     """ember_kv_batch (include/ember_attn.h)."""
 
+    device = None  # of its arrays, set by kv_batch
     _fields_ = [("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_q", ctypes.c_int), ("max_kv", ctypes.c_int),
                 ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p),
                 ("max_pages", ctypes.c_int), ("shared", ctypes.c_int)]
@@ -33,6 +34,7 @@ class KvBatch(ctypes.Structure):
 class AttnOpts(ctypes.Structure):
     """ember_attn_opts (include/ember_attn.h)."""
 
+    device = None  # of its arrays, set by attn_options
     _fields_ = [("n_heads", ctypes.c_int), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
                 ("window", ctypes.c_int), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
 
@@ -61,14 +63,17 @@ def type_id(t) -> int:
     return ty
 
 
-def on_current_device(*tensors) -> int:
-    """Refuses tensors that are not on the current device, where the library launches; its index."""
+def on_current_device(*tensors, made=()) -> int:
+    """Refuses tensors, and descriptors `made` of some, that are not on the current device, where the library launches; its index."""
     import torch
 
     here = torch.cuda.current_device()
     for t in tensors:
         if t.get_device() != here:  # (-1 for a CPU tensor)
             raise em.EmberError(em.ERR_LAUNCH, f"tensor on {t.device}, the current device is cuda:{here}")
+    for d in made:
+        if d.device is not None and d.device != here:
+            raise em.EmberError(em.ERR_LAUNCH, f"{type(d).__name__} on cuda:{d.device}, the current device is cuda:{here}")
     return here
 
 
@@ -102,8 +107,8 @@ def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: int = 
         if pages.dim() != 2 or pages.shape[0] < n:
             raise em.EmberError(em.ERR_SHAPE, "pages: [n_seqs, max_pages] is needed")
         b.pages, b.max_pages = _array(pages, pages.numel(), torch.int32, "pages"), pages.shape[1]
-    on_current_device(*(t for t in (kv_len, q_start, pages) if t is not None))
-    b._owner = (kv_len, q_start, pages)  # (all on one device: calls look at the first's)
+    b.device = on_current_device(*(t for t in (kv_len, q_start, pages) if t is not None))
+    b._owner = (kv_len, q_start, pages)
     return b
 
 
@@ -115,7 +120,8 @@ def attn_options(n_heads: int, head_dim: int, scale: Optional[float] = None, sof
     a = AttnOpts(n_heads=n_heads, scale=head_dim ** -0.5 if scale is None else scale, softcap=softcap, window=window)
     a.slopes = _array(slopes, n_heads, torch.float32, "slopes")
     a.prefix = _array(prefix, 0, torch.int32, "prefix")
-    on_current_device(*(t for t in (slopes, prefix) if t is not None))
+    if slopes is not None or prefix is not None:
+        a.device = on_current_device(*(t for t in (slopes, prefix) if t is not None))
     a._owner = (slopes, prefix)
     return a
 
@@ -155,7 +161,7 @@ class DeviceKvCache:
         d = self.desc
         d.type, (d.n_pages, d.n_kv, d.page, d.head_dim) = self.type, shape
         d.k, d.v = self.k.data_ptr(), self.v.data_ptr()
-        on_current_device(self.k, self.v)
+        self.device = on_current_device(self.k, self.v)
         if self.type == em.Q8_0:
             for t in (self.k_scale, self.v_scale):
                 if t is None or tuple(t.shape) != shape[:3] + (shape[3] // 32,) or t.dtype != torch.float16 or not t.is_contiguous():
@@ -183,7 +189,7 @@ class DeviceKvCache:
         ty = type_id(k)
         if k.dtype != v.dtype:
             raise em.EmberError(em.ERR_TYPE, "k and v of one type are needed")
-        here = on_current_device(k, v, self.k, *getattr(batch, "_owner", ())[:1])
+        here = on_current_device(k, v, made=(self, batch))
         st = getattr(em.lib(), fn)(ctypes.byref(d), ctypes.byref(batch), k.data_ptr(), ks, v.data_ptr(), vs, ty, em._stream(stream, here))
         if st:
             raise em.EmberError(st, fn)
@@ -206,14 +212,14 @@ class DeviceKvCache:
 
         d = self.desc
         qs = _rows(q, batch.n_tokens, opts.n_heads, d.head_dim, "q")
-        here = on_current_device(q, self.k, *getattr(batch, "_owner", ())[:1])
+        here = torch.cuda.current_device()
         if out is None:
             own_stream(stream, here, "out")
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         os_ = _rows(out, batch.n_tokens, opts.n_heads, d.head_dim, "out")
         if out.dtype != q.dtype:
             raise em.EmberError(em.ERR_TYPE, "q and out of one type are needed")
-        slopes, prefix = getattr(opts, "_owner", (None, None))
+        prefix = getattr(opts, "_owner", (None, None))[1]
         if prefix is not None and prefix.numel() < batch.n_seqs:
             raise em.EmberError(em.ERR_SHAPE, "prefix: one length per sequence is needed")
         if scratch is None:
@@ -223,7 +229,7 @@ class DeviceKvCache:
             scratch = torch.empty(max(1, need), dtype=torch.uint8, device=q.device)
         elif not scratch.is_contiguous():
             raise em.EmberError(em.ERR_SCRATCH, "scratch: contiguous memory is needed")
-        on_current_device(out, scratch, *(t for t in (slopes, prefix) if t is not None))
+        on_current_device(q, out, scratch, made=(self, batch, opts))
         st = em.lib().ember_attn(ctypes.byref(opts), ctypes.byref(d), ctypes.byref(batch), q.data_ptr(), qs, out.data_ptr(), os_,
                                  type_id(q), scratch.data_ptr(), scratch.numel() * scratch.element_size(), em._stream(stream, here))
         if st:
