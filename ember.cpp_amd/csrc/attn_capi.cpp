@@ -57,6 +57,7 @@ int check_attn(const ember_attn_opts* a, const ember_kv_cache* c, const ember_kv
   if ((s = check_cache(c)) || (s = check_batch(c, b))) return s;
   if (a->n_heads < 1 || a->n_heads % c->n_kv || a->n_heads / c->n_kv > 128) return EMBER_ERR_SHAPE;
   if (!(a->scale > 0.0f) || !(a->scale < 1e30f) || !(a->softcap >= 0.0f) || !(a->softcap < 1e30f) || a->window < 0) return EMBER_ERR_SHAPE;
+  if (a->softcap > 0.0f && !(a->scale / a->softcap < 1e30f)) return EMBER_ERR_SHAPE;  // (a quotient that the kernels multiply by)
   if (!aligned(a->slopes, 4) || !aligned(a->prefix, 4)) return EMBER_ERR_ALIGN;
   return EMBER_OK;
 }

@@ -93,14 +93,20 @@ def _array(t, n: int, dtype, what: str) -> int:
     return t.data_ptr()
 
 
-def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: int = 1, max_kv: int = 0, pages=None,
-             shared: int = 0) -> KvBatch:
+def kv_batch(kv_len, q_start=None, n_tokens: Optional[int] = None, max_q: Optional[int] = None, max_kv: Optional[int] = None,
+             pages=None, shared: int = 0) -> KvBatch:
     """A batch's descriptor from int32 device tensors: kv_len [n_seqs], q_start [n_seqs + 1] (None: one new token
-    each), pages [n_seqs, max_pages] (None: sequence b lies in page b). Keeps the tensors."""
+    each), pages [n_seqs, max_pages] (None: sequence b lies in page b). max_kv, the most tokens that a sequence has, is needed, and with
+    q_start n_tokens; max_q None: n_tokens (of one sequence). Keeps the tensors."""
     import torch
 
     n = kv_len.numel()
-    b = KvBatch(n_seqs=n, n_tokens=n if n_tokens is None else n_tokens, max_q=max_q, max_kv=max_kv, shared=shared)
+    if max_kv is None or (q_start is not None and n_tokens is None):
+        raise em.EmberError(em.ERR_SHAPE, "max_kv, and n_tokens with q_start, are needed")
+    n_tokens = n if n_tokens is None else n_tokens
+    if max_q is None:
+        max_q = 1 if q_start is None else max(n_tokens, 1)
+    b = KvBatch(n_seqs=n, n_tokens=n_tokens, max_q=max_q, max_kv=max_kv, shared=shared)
     b.kv_len = _array(kv_len, n, torch.int32, "kv_len")
     b.q_start = _array(q_start, n + 1, torch.int32, "q_start")
     if pages is not None:

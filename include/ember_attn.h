@@ -49,7 +49,7 @@ typedef struct ember_kv_cache {
  * No two rows of a call may have the same place in the cache where the call stores them. */
 typedef struct ember_kv_batch {
   int n_seqs;               /* up to 65535 */
-  int n_tokens;             /* rows of q, k, v and out */
+  int n_tokens;             /* rows of q, k, v and out; calls of over 2^24 blocks (of 128 rows of a KV head, or 8 KB) are refused */
   int max_q;                /* no sequence has more new tokens (those past max_q get no attention output) */
   int max_kv;               /* no sequence has more tokens in the cache; up to 1 << 29 */
   const int32_t* q_start;   /* [n_seqs + 1] device, ascending, or NULL: one token each, n_tokens >= n_seqs */
@@ -79,11 +79,11 @@ int ember_kv_load(const ember_kv_cache* c, const ember_kv_batch* b, void* k, int
  *   s = scale * (q . k_j);  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s -= slopes[h] * |p - j|
  * and the output row the softmax-weighted sum of the visible keys' values, zeros if no key is visible. Keys and
  * values that a row does not see have no effect on it, whatever they hold; a row that sees one that is infinite or NaN is
- * not finite in the columns that hold it, or in all. */
+ * not finite in the columns that hold it, or in all. Scores are f32 and have to stay within +-1e29. */
 typedef struct ember_attn_opts {
   int n_heads;           /* a multiple of n_kv, up to 128 per KV head */
   float scale;           /* > 0 */
-  float softcap;         /* 0: none */
+  float softcap;         /* 0: none; else over scale * 1e-30 */
   int window;            /* 0: none */
   const float* slopes;   /* [n_heads] device, or NULL */
   const int32_t* prefix; /* [n_seqs] device, or NULL */

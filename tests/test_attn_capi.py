@@ -140,3 +140,16 @@ def test_places_and_plans():
     assert os.path.exists(exe), f"{exe} is missing: run `make` in ember.cpp_amd/"
     r = subprocess.run([exe], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.startswith("ok"), r.stdout + r.stderr
+
+
+def test_a_cap_far_under_the_scale_is_refused():
+    assert _attn(opts(softcap=1e-39), cache(), batch()) == em.ERR_SHAPE
+    assert _attn(opts(softcap=1e-35, scale=1.0), cache(), batch()) == em.ERR_SHAPE
+
+
+def test_a_batch_needs_its_sizes():
+    torch = pytest.importorskip("torch")
+    for kw in (dict(), dict(max_kv=5, q_start=torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(em.EmberError) as e:
+            em.kv_batch(torch.ones(1, dtype=torch.int32), **kw)
+        assert e.value.status == em.ERR_SHAPE
