@@ -49,7 +49,8 @@ typedef struct ember_kv_cache {
  * No two rows of a call may have the same place in the cache where the call stores them. */
 typedef struct ember_kv_batch {
   int n_seqs;               /* up to 65535 */
-  int n_tokens;             /* rows of q, k, v and out; calls of over 2^24 blocks (of 128 rows of a KV head, or 8 KB) are refused */
+  int n_tokens;             /* rows of q, k, v and out. A call too large for a launch (2^24 blocks: of 128 rows of a KV head in the
+                             * attention, of 8192 values in store and load) is refused with EMBER_ERR_SHAPE */
   int max_q;                /* no sequence has more new tokens (those past max_q get no attention output) */
   int max_kv;               /* no sequence has more tokens in the cache; up to 1 << 29 */
   const int32_t* q_start;   /* [n_seqs + 1] device, ascending, or NULL: one token each, n_tokens >= n_seqs */
