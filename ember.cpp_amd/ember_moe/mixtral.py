@@ -24,10 +24,9 @@ from __future__ import annotations
 
 import time
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
-
-from typing import Optional
 
 from . import (DeviceKvCache, EmberError, Layer, Q4_K, Sampler, TYPE_NAMES, _ptr, attn_options, kv_batch, moe_ffn,
                prefill_pack, prefill_pack_bytes, quantize, sample, scratch_bytes)
